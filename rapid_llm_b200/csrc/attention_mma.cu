@@ -24,6 +24,7 @@
 // reference's tensor-core kernels do (flashattention2_nopad.py:162).
 #include <mutex>
 
+#include "attention_shared.h"
 #include "attention_static_scratch.h"
 #include "common.cuh"
 
@@ -78,6 +79,10 @@ struct AttentionArgs {
   int gate_stride;
   int kv_planes;            // 2; or 1 for a cache [num_pages, 1, hkv, page_size, D] whose rows are keys and values at once
                             // (the mma.sync tiles only)
+  // Listed items (attention over shared prefixes, attention_shared.h): `items` holds eight numbers an item.
+  const int* members;       // the tokens an item's rows belong to
+  const int* positions;     // [tokens]
+  const int* part_first;    // [tokens + 1]  a token's first place among the parts
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -119,7 +124,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // kShared: the cache has one plane, a row is key and value at once, and a block's rows are brought to shared
 // memory once and read as both (half the copies, half the stages' memory, so two CTAs fit on an SM at any head size).
 // kSloped: a slope per head times the distance between query and key is taken off the score.
-template <int kWarpsM, int kWarpsN, int kStages, bool kShared, bool kSloped>
+// kListed: an item names its rows' tokens and its key range itself and leaves a part of each row's result (attention_shared.h).
+template <int kWarpsM, int kWarpsN, int kStages, bool kShared, bool kSloped, bool kListed = false>
 __global__ void __launch_bounds__(kThreads)
 attention_mma_kernel(const AttentionArgs args) {
   static_assert(kWarpsM * kWarpsN == 4, "four warps");
@@ -136,14 +142,18 @@ attention_mma_kernel(const AttentionArgs args) {
   const int wm = warp % kWarpsM, wn = warp / kWarpsM;
   // the kv head is the fast grid dimension: CTAs start in the order of the item list (longest
   // first) over all heads, so the last wave holds the shortest items
-  const int* item = args.items + static_cast<size_t>(blockIdx.y) * 4;
-  const int entry = item[0], row0 = item[1], split = item[2];
+  const int* item = args.items + static_cast<size_t>(blockIdx.y) * (kListed ? kListedInts : 4);
+  const int entry = item[0];
+  const int row0 = kListed ? item[kListedRow0] : item[1], split = kListed ? item[kListedPart] : item[2];
   const int kv_head = blockIdx.x;
   const int group = args.hq / args.hkv;
-  const int tok_begin = args.cu_seqlens[entry];
-  const int n_rows = (args.cu_seqlens[entry + 1] - tok_begin) * group;
-  const int start = args.entry_start[entry];
+  const int tok_begin = kListed ? 0 : args.cu_seqlens[entry];
+  const int n_rows = kListed ? row0 + item[kListedRows] : (args.cu_seqlens[entry + 1] - tok_begin) * group;
+  const int start = kListed ? 0 : args.entry_start[entry];
   const int slot = args.entry_slot[entry];
+  const int* members = kListed ? args.members + item[kListedMembers] : nullptr;
+  // the token (a row of q) that place `token` of the item or entry stands for
+  auto token_at = [&](int token) { return kListed ? members[token] : tok_begin + token; };
 
   // rows of this thread in the accumulator layout: r_a = lane / 4 and r_a + 8 of its warp
   int row_pos[2], row_lo[2], row_token[2], row_head[2];
@@ -153,10 +163,16 @@ attention_mma_kernel(const AttentionArgs args) {
     const int p = row0 + wm * 16 + (lane >> 2) + 8 * i;
     row_valid[i] = p < n_rows;
     const int token = p / group;
-    row_token[i] = tok_begin + token;
     row_head[i] = kv_head * group + (p - token * group);
-    row_pos[i] = row_valid[i] ? start + token : -1;
-    row_lo[i] = first_visible(row_pos[i], args.window, args.chunk);
+    if constexpr (kListed) {
+      row_token[i] = row_valid[i] ? members[token] : 0;
+      row_pos[i] = row_valid[i] ? args.positions[row_token[i]] : -1;
+      row_lo[i] = item[kListedFirst];
+    } else {
+      row_token[i] = tok_begin + token;
+      row_pos[i] = row_valid[i] ? start + token : -1;
+      row_lo[i] = first_visible(row_pos[i], args.window, args.chunk);
+    }
   }
   float slope_log2[2] = {0.0f, 0.0f};
   if constexpr (kSloped) {
@@ -166,7 +182,14 @@ attention_mma_kernel(const AttentionArgs args) {
   }
 
   const int last_row = min(n_rows, row0 + kTileM) - 1;
-  const int min_pos = start + row0 / group, max_pos = start + last_row / group;
+  if constexpr (kListed) {
+    if (last_row < row0) {       // a place of the list that holds no item
+      pdl_wait();
+      return;
+    }
+  }
+  const int min_pos = kListed ? item[kListedFirst] : start + row0 / group;
+  const int max_pos = kListed ? item[kListedEnd] - 1 : start + last_row / group;
   bool bad = slot < 0 || slot >= args.slots || start < 0 ||
              max_pos >= args.max_pages * args.page_size || last_row < row0;
   if (bad) {
@@ -174,12 +197,12 @@ attention_mma_kernel(const AttentionArgs args) {
   }
   // key range of the tile, then of this split (begin on a multiple of 64)
   const int hi = bad ? 0 : max_pos + 1;
-  const int lo = first_visible(min_pos, args.window, args.chunk);
+  const int lo = kListed ? min_pos : first_visible(min_pos, args.window, args.chunk);
   const int lo_aligned = lo & ~(kBlockN - 1);
   const int span = max(hi - lo_aligned, 0);
   const int per_split = ((span + args.splits - 1) / args.splits + kBlockN - 1) / kBlockN * kBlockN;
-  const int k_begin = lo_aligned + split * per_split;
-  const int k_end = min(hi, k_begin + per_split);
+  const int k_begin = kListed ? lo_aligned : lo_aligned + split * per_split;
+  const int k_end = kListed ? hi : min(hi, k_begin + per_split);
   const int n_blocks = k_end > k_begin ? (k_end - k_begin + kBlockN - 1) / kBlockN : 0;
   const int* table = args.block_table + static_cast<size_t>(bad ? 0 : slot) * args.max_pages;
   const size_t v_plane = args.kv_planes == 2 ? static_cast<size_t>(args.hkv) * args.page_size * kD : 0;
@@ -212,7 +235,7 @@ attention_mma_kernel(const AttentionArgs args) {
       const int token = p / group;
       const bf16* src = args.q;
       if (valid)
-        src = args.q + (static_cast<size_t>(tok_begin + token) * args.hq + kv_head * group +
+        src = args.q + (static_cast<size_t>(token_at(token)) * args.hq + kv_head * group +
                         (p - token * group)) * kD + c * 8;
       cp_async16(smem_u32(q_smem + r * kStride + c * 8), src, valid);
     }
@@ -427,6 +450,15 @@ attention_mma_kernel(const AttentionArgs args) {
     for (int i = 0; i < 2; ++i) {
       if (!row_valid[i]) continue;
       float inv = run_sum[i] > 0.0f ? 1.0f / run_sum[i] : 0.0f;
+      if constexpr (kListed) {
+        const size_t at = static_cast<size_t>(args.part_first[row_token[i]] + split) * args.hq + row_head[i];
+        float* dst = args.part_out + at * kD + (lane & 3) * 2;
+#pragma unroll
+        for (int nt = 0; nt < kD / 8; ++nt)
+          *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(o_acc[nt][2 * i] * inv, o_acc[nt][2 * i + 1] * inv);
+        if ((lane & 3) == 0) args.part_lse[at] = run_sum[i] > 0.0f ? run_max[i] + log2f(run_sum[i]) : -INFINITY;
+        continue;
+      }
       const size_t row = static_cast<size_t>(row_token[i]) * args.hq + row_head[i];
       if (args.splits == 1 && args.sink != nullptr) {
         // the sink joins the denominator of an unsplit row here (of a split one in the merge kernel)
@@ -490,6 +522,12 @@ attention_mma_kernel(const AttentionArgs args) {
       }
       float inv = total > 0.0f ? 1.0f / total : 0.0f;
       const int token = p / group, head = kv_head * group + (p - token * group);
+      if constexpr (kListed) {
+        const size_t at = static_cast<size_t>(args.part_first[members[token]] + split) * args.hq + head;
+        args.part_out[at * kD + c] = value * inv;
+        if (c == 0) args.part_lse[at] = total > 0.0f ? m + log2f(total) : -INFINITY;
+        continue;
+      }
       const size_t row = static_cast<size_t>(tok_begin + token) * args.hq + head;
       if (args.splits == 1 && args.sink != nullptr) {
         const float sink2 = args.sink[head] * 1.4426950408889634f;
@@ -546,9 +584,9 @@ constexpr size_t attention_smem_bytes() {
   return static_cast<size_t>(16 * kWarpsM + (kShared ? 1 : 2) * kStages * kBlockN) * kStride * sizeof(bf16);
 }
 
-template <int kWarpsM, int kWarpsN, int kStages, bool kShared, bool kSloped>
+template <int kWarpsM, int kWarpsN, int kStages, bool kShared, bool kSloped, bool kListed = false>
 int launch_attention_as(const AttentionArgs& args, int n_items, bool pdl, cudaStream_t stream) {
-  auto kernel = attention_mma_kernel<kWarpsM, kWarpsN, kStages, kShared, kSloped>;
+  auto kernel = attention_mma_kernel<kWarpsM, kWarpsN, kStages, kShared, kSloped, kListed>;
   constexpr size_t smem = attention_smem_bytes<kWarpsM, kWarpsN, kStages, kShared>();
   static_assert(smem <= 227 * 1024, "shared memory of one CTA");
   static std::atomic<unsigned long long> configured;   // one per instantiation and per library image
@@ -869,6 +907,54 @@ int rl_attention_mma(const void* q, const void* cache, void* out, float* part_ou
                                out_stride, static_cast<const attn::bf16*>(gate), gate_stride);
   }
   return status;
+}
+
+// Attention over shared prefixes (attention_shared.h): tile_items of up to tile_rows packed rows, row_items of up to 16,
+// [n, 8] int32 each, then the join.  tile_rows: 64 = the mma.sync tiles.
+int rl_attention_shared(const void* q, const void* cache, void* out, float* part_out, float* part_lse, const int* tile_items,
+                        int n_tile_items, int tile_rows, const int* row_items, int n_row_items, int most_rows,
+                        const int* members, const int* positions, const int* part_first, const int* entry_slot,
+                        const int* block_table, int tokens, int hq, int hkv, int head_dim, int page_size, int num_pages,
+                        int max_pages, int slots, float scale, const float* sink, const float* slopes, int out_stride,
+                        const void* gate, int gate_stride, int* fault, int pdl, cudaStream_t stream) {
+  if (tokens == 0) return 0;
+  if (head_dim != attn::kD || hkv <= 0 || hq % hkv != 0 || page_size <= 0 || hkv > 65535 || n_tile_items < 0 || n_row_items < 0 ||
+      n_tile_items > 65535 || n_row_items > 65535 || tile_rows != 64 || out_stride < hq * head_dim || out_stride % 8 != 0 ||
+      (reinterpret_cast<uintptr_t>(out) & 15) || (gate != nullptr && gate_stride < hq) ||
+      static_cast<long long>(tokens) * hq > 0x7fffffffll)
+    return static_cast<int>(cudaErrorInvalidValue);
+  attn::AttentionArgs args = {};
+  args.q = static_cast<const attn::bf16*>(q);
+  args.cache = static_cast<const attn::bf16*>(cache);
+  args.part_out = part_out;
+  args.part_lse = part_lse;
+  args.entry_slot = entry_slot;
+  args.block_table = block_table;
+  args.hq = hq; args.hkv = hkv; args.page_size = page_size; args.num_pages = num_pages;
+  args.max_pages = max_pages; args.slots = slots; args.splits = 1;
+  args.scale = scale;
+  args.scale_log2 = scale * 1.4426950408889634f;
+  args.slopes = slopes; args.kv_planes = 2;
+  args.members = members; args.positions = positions; args.part_first = part_first;
+  args.fault = fault;
+  int status = 0;
+  if (n_tile_items > 0) {
+    args.items = tile_items;
+    status = slopes != nullptr ? attn::launch_attention_as<4, 1, 2, false, true, true>(args, n_tile_items, pdl != 0, stream)
+                               : attn::launch_attention_as<4, 1, 2, false, false, true>(args, n_tile_items, pdl != 0, stream);
+    if (status != 0) return status;
+  }
+  if (n_row_items > 0) {
+    args.items = row_items;
+    status = slopes != nullptr ? attn::launch_attention_as<1, 4, 3, false, true, true>(args, n_row_items, pdl != 0, stream)
+                               : attn::launch_attention_as<1, 4, 3, false, false, true>(args, n_row_items, pdl != 0, stream);
+    if (status != 0) return status;
+  }
+  const int rows = tokens * hq;
+  return rl::launch_kernel(rl::attention_join_kernel<attn::bf16>, dim3((rows + rl::kJoinWarps - 1) / rl::kJoinWarps),
+                           dim3(rl::kJoinWarps * 32), 0, stream, pdl != 0, part_out, part_lse, part_first,
+                           static_cast<attn::bf16*>(out), rows, hq, head_dim, out_stride, sink,
+                           static_cast<const attn::bf16*>(gate), gate_stride);
 }
 
 }  // extern "C"

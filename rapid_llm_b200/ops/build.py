@@ -42,6 +42,7 @@ LIBRARIES: dict[str, list[str]] = {
         "elementwise.cu",
         "rope_kv.cu",
         "attention_generic.cu",
+        "attention_shared_f32.cu",
         "gemm_f32.cu",
         "gemm_f32_split.cu",
         "sampling.cu",

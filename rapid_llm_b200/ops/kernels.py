@@ -143,6 +143,11 @@ def core() -> ctypes.CDLL:
             c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
             c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
         ]
+        lib.rl_attention_shared_f32.argtypes = [
+            c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+            c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p,
+            c_int, c_void_p,
+        ]
         lib.rl_embedding_sum.argtypes = [
             c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
             c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_int, c_float,
@@ -158,7 +163,7 @@ def core() -> ctypes.CDLL:
         for name in (
             "rl_embedding", "rl_embedding_sum", "rl_scatter_rows", "rl_add_rmsnorm", "rl_silu_mul", "rl_to_float", "rl_clamped_glu",
             "rl_rope_unit_write", "rl_layernorm", "rl_row_norm_rope_write", "rl_sigmoid_gate", "rl_relu_squared",
-            "rl_qk_norm_rope_write", "rl_attention_generic", "rl_gemm_f32", "rl_sample",
+            "rl_qk_norm_rope_write", "rl_attention_generic", "rl_attention_shared_f32", "rl_gemm_f32", "rl_sample",
         ):
             getattr(lib, name).restype = c_int
         _SIGNATURES_SET = True
@@ -632,6 +637,12 @@ def attention_lib(head_dim: int) -> ctypes.CDLL:
             c_int, c_int, c_void_p, c_int, c_void_p,
         ]
         lib.rl_attention_mma.restype = c_int
+        lib.rl_attention_shared.argtypes = [
+            c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p,
+            c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p,
+            c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
+        ]
+        lib.rl_attention_shared.restype = c_int
         lib.rl_attention_decode_max_clusters.argtypes = [c_int]
         lib.rl_attention_decode_max_clusters.restype = c_int
         if lib.rl_attention_head_dim() != head_dim:
@@ -754,6 +765,90 @@ def attention_mma(
         f"attention_mma(head_dim={head_dim})",
     )
     LAUNCHES.count += (1 if n_chunk and n_decode else 0) + (1 if splits > 1 else 0)
+    return out
+
+
+SHARED_F32_ROWS = 32      # packed rows of an item of the float32 kernel over shared prefixes
+SHARED_ITEM = 8           # numbers that describe an item
+
+
+def attention_shared(
+    q: torch.Tensor,
+    cache: torch.Tensor,
+    out: torch.Tensor,
+    *,
+    plan: dict,
+    part_out: torch.Tensor | None,
+    part_lse: torch.Tensor | None,
+    positions: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    entry_start: torch.Tensor,
+    entry_slot: torch.Tensor,
+    block_table: torch.Tensor,
+    num_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    scale: float,
+    fault: torch.Tensor,
+    sink: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    slopes: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Causal attention of a step's tokens over their requests' cached keys, where groups of requests share the pages of their
+    first positions: those are read once for the whole group.  The result is that of :func:`attention_mma` /
+    :func:`attention_generic` over each request's own block table.
+
+    ``plan`` is what ``parts.attention.SharedItems.plan`` made of the step, its arrays on the device; it says which entries share
+    how many positions, and the block tables of a group's entries must name the same pages there.  ``part_out``
+    ``[part_rows, head_dim]`` and ``part_lse`` ``[part_rows]`` (float32) are scratch of ``SharedItems.part_rows(plan)`` rows
+    and more; calls that may run at the same time need scratch of their own.  ``sink``, ``gate`` and ``slopes`` as in :func:`attention_mma`, rows of ``out`` and
+    ``gate`` too; every key up to a token's own position is seen (no window, no squashed scores, caches of two planes)."""
+    _need_cuda(q, cache, out, part_out, part_lse, positions, cu_seqlens, entry_start, entry_slot, block_table, fault, sink, gate, slopes)
+    _per_head(num_heads, sink=sink, slopes=slopes)
+    _contig("q", q), _contig("cache", cache)
+    for name, tensor in (("positions", positions), ("cu_seqlens", cu_seqlens), ("entry_start", entry_start),
+                         ("entry_slot", entry_slot), ("block_table", block_table), ("fault", fault)):
+        _expect(name, tensor, torch.int32), _contig(name, tensor)
+    tokens, width = positions.numel(), num_heads * head_dim
+    if cache.dim() != 5 or cache.shape[1] != 2 or cache.shape[2] != num_kv_heads or cache.shape[4] != head_dim or num_heads % num_kv_heads:
+        raise KernelError("attention: cache must be [pages, 2, kv_heads, page_size, head_dim], heads a multiple of kv heads")
+    if q.shape != (tokens, width) or out.shape != q.shape or cache.dtype != q.dtype or out.dtype != q.dtype:
+        raise KernelError("attention: q and out must be [tokens, heads * head_dim] of the cache's dtype")
+    if plan["tokens"] != tokens or plan["heads"] != (num_heads // num_kv_heads, num_kv_heads, head_dim) or plan["dtype"] != dtype_tag(q.dtype):
+        raise KernelError("attention: the plan was made for another step")
+    if plan["entries"] != entry_slot.numel() or block_table.dim() != 2:
+        raise KernelError("attention: the plan was made for another number of entries")
+    out_stride, gate_stride = _attention_out(out, gate, tokens, num_heads, head_dim)
+    tile_items, row_items = plan["tile_items"], plan["row_items"]
+    members, part_first = plan["members"], plan["part_first"]
+    _need_cuda(tile_items, row_items, members, part_first)
+    for name, tensor in (("tile_items", tile_items), ("row_items", row_items), ("members", members), ("part_first", part_first)):
+        _expect(name, tensor, torch.int32), _contig(name, tensor)
+    need = plan["parts"] * num_heads
+    _expect("part_out", part_out, torch.float32), _expect("part_lse", part_lse, torch.float32)
+    if part_out is None or part_lse is None or part_out.numel() < need * head_dim or part_lse.numel() < need:
+        raise KernelError("attention: scratch for the parts is missing or too small")
+    _contig("part_out", part_out), _contig("part_lse", part_lse)
+    if q.dtype == torch.float32:
+        launches = 1 + (tile_items.numel() > 0)
+        _check(
+            core().rl_attention_shared_f32(
+                _ptr(q), _ptr(cache), _ptr(out), _ptr(part_out), _ptr(part_lse), _ptr(tile_items), tile_items.numel() // SHARED_ITEM,
+                _ptr(members), _ptr(positions), _ptr(part_first), _ptr(entry_slot), _ptr(block_table), tokens, num_heads,
+                num_kv_heads, head_dim, cache.shape[3], cache.shape[0], block_table.shape[1], block_table.shape[0], float(scale),
+                _ptr(sink), _ptr(slopes), out_stride, _ptr(gate), gate_stride, _ptr(fault), int(PDL), _stream()),
+            f"attention_shared(head_dim={head_dim})")
+    else:
+        launches = 1 + (tile_items.numel() > 0) + (row_items.numel() > 0)
+        _check(
+            attention_lib(head_dim).rl_attention_shared(
+                _ptr(q), _ptr(cache), _ptr(out), _ptr(part_out), _ptr(part_lse), _ptr(tile_items), tile_items.numel() // SHARED_ITEM,
+                plan["tile_rows"], _ptr(row_items), row_items.numel() // SHARED_ITEM, plan["most_rows"], _ptr(members),
+                _ptr(positions), _ptr(part_first), _ptr(entry_slot), _ptr(block_table), tokens, num_heads, num_kv_heads, head_dim,
+                cache.shape[3], cache.shape[0], block_table.shape[1], block_table.shape[0], float(scale), _ptr(sink), _ptr(slopes),
+                out_stride, _ptr(gate), gate_stride, _ptr(fault), int(PDL), _stream()),
+            f"attention_shared(head_dim={head_dim})")
+    LAUNCHES.count += launches - 1
     return out
 
 

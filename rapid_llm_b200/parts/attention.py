@@ -230,6 +230,93 @@ class AttentionItems(StepPlanner):
                 "chunk_rows": int(chunk_rows)}
 
 
+class SharedItems(StepPlanner):
+    """Cuts a step whose requests share prefixes into the work items of ``kernels.attention_shared``.
+
+    ``shape.prefix_group`` and ``shape.prefix_tokens`` say which entries share how many of their first positions.  A group's
+    shared keys become items over the packed rows (token, head of the group) of all its members, every entry's other keys items
+    over its own rows; rows beyond a tile's are further items, and key ranges are cut until the items fill the GPU.
+    An item is eight numbers (``csrc/attention_shared.h``).  Items of more than 16 rows are tiles, the others rows; the
+    float32 kernel takes one kind.
+    """
+
+    def __init__(self, group: int, num_kv_heads: int, head_dim: int, sms: int = DEFAULT_SMS, dtype: torch.dtype = torch.bfloat16) -> None:
+        self.group, self.num_kv_heads, self.head_dim, self.sms = int(group), int(num_kv_heads), int(head_dim), int(sms)
+        self.wide = dtype == torch.float32
+        self.tag = kernels.dtype_tag(dtype)
+        self.key = ("shared_items", self.group, self.num_kv_heads, self.head_dim, self.sms, self.tag)
+
+    def part_rows(self, plan: dict) -> int:
+        """Rows of the two scratch buffers."""
+        return plan["parts"] * self.group * self.num_kv_heads
+
+    def plan(self, shape: StepShape) -> dict:
+        lengths, starts = np.asarray(shape.lengths, dtype=np.int64), np.asarray(shape.starts, dtype=np.int64)
+        count = len(lengths)
+        groups = np.full(count, -1, dtype=np.int64) if shape.prefix_group is None else np.asarray(shape.prefix_group, dtype=np.int64)
+        shared = np.zeros(count, dtype=np.int64) if shape.prefix_tokens is None else np.asarray(shape.prefix_tokens, dtype=np.int64)
+        if groups.shape != lengths.shape or shared.shape != lengths.shape or starts.shape != lengths.shape or (lengths < 1).any():
+            raise ValueError("a step has one length (of at least one token), start, group and number of shared positions per entry")
+        shared = np.where(groups >= 0, shared, 0)
+        if (shared < 0).any() or (shared > starts).any():
+            raise ValueError("shared positions must lie before an entry's new tokens")
+        first_token = np.concatenate(([0], np.cumsum(lengths)))
+        tokens = int(first_token[-1])
+        members = [np.arange(tokens, dtype=np.int64)]           # an entry's own rows, then each group's
+        at = tokens
+        block = kernels.DECODE_TC_KEYS
+        work = []                                               # entry, first key, end, first member, rows, fresh key, tokens
+        for number in np.unique(groups[(groups >= 0) & (shared > 0)]):
+            inside = np.flatnonzero(groups == number)
+            if (shared[inside] != shared[inside[0]]).any():
+                raise ValueError("the entries of a group share one number of positions")
+            its = np.concatenate([np.arange(first_token[e], first_token[e + 1]) for e in inside])
+            members.append(its)
+            keys = int(shared[inside[0]])
+            work.append((int(inside[0]), 0, keys, at, len(its), keys, its))
+            at += len(its)
+        for entry in range(count):
+            its = np.arange(first_token[entry], first_token[entry + 1])
+            work.append((entry, int(shared[entry]), int(starts[entry] + lengths[entry]), int(first_token[entry]), len(its),
+                         int(starts[entry]), its))
+
+        tile_rows = kernels.SHARED_F32_ROWS if self.wide else kernels.CHUNK_TILE_ROWS
+
+        def rows_of(rows: int) -> int:
+            return tile_rows if self.wide or rows > kernels.DECODE_TILE_ROWS else kernels.DECODE_TILE_ROWS
+
+        units = sum(-(-(end - first) // block) * -(-n * self.group // rows_of(n * self.group))
+                    for _, first, end, _, n, _, _ in work) * self.num_kv_heads
+        ctas = 2 * self.sms
+        per_item = max(1, -(-units // ctas))                    # blocks of keys an item takes
+        parts = np.zeros(tokens, dtype=np.int64)                # of each token so far: a group's items come before its entries'
+        tiles, rows, most = [], [], 0
+        for entry, first, end, member, n, fresh, its in work:
+            packed = n * self.group
+            height = rows_of(packed)
+            bucket = tiles if height == tile_rows else rows
+            if bucket is rows:
+                most = max(most, min(height, packed))
+            ranges = max(1, -(-(end - first) // (per_item * block)))
+            step = -(-(-(-(end - first) // ranges)) // block) * block
+            lows = range(first, end, step)
+            offset = int(parts[its[0]])
+            for index, low in enumerate(lows):
+                for row0 in range(0, packed, height):
+                    bucket.append((entry, low, min(low + step, end), member, row0, min(height, packed - row0), offset + index, fresh))
+            parts[its] += len(lows)
+
+        def listed(bucket) -> np.ndarray:
+            items = np.asarray(bucket, dtype=np.int32).reshape(-1, kernels.SHARED_ITEM)
+            return np.ascontiguousarray(items[np.argsort(items[:, 1] - items[:, 2], kind="stable")])      # the longest first
+
+        part_first = np.concatenate(([0], np.cumsum(parts)))
+        return {"tile_items": listed(tiles), "row_items": listed(rows), "members": np.concatenate(members).astype(np.int32),
+                "part_first": part_first.astype(np.int32), "parts": int(part_first[-1]), "tokens": tokens, "entries": count,
+                "tile_rows": int(tile_rows), "most_rows": int(most), "heads": (self.group, self.num_kv_heads, self.head_dim),
+                "dtype": self.tag}
+
+
 @MIXERS.register("gqa_attention")
 class GQAAttention(Mixer):
     rides_norms = True

@@ -120,6 +120,10 @@ class StepShape:
     decode_only: bool
     page_size: int = 0    # tokens per cache page (0 = not said)
     padding: int = 0      # how many of the entries, at the end, are padding rows
+    # entries that share the pages of their first positions: per entry its group's number (-1 = none) and how many
+    # positions the group shares; None = nothing is shared
+    prefix_group: Any = None      # numpy int32 [entries]
+    prefix_tokens: Any = None     # numpy int32 [entries]
 
 
 class StepPlanner:
