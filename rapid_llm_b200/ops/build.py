@@ -43,9 +43,11 @@ LIBRARIES: dict[str, list[str]] = {
         "rope_kv.cu",
         "attention_generic.cu",
         "attention_shared_f32.cu",
+        "cache_pages.cu",
         "gemm_f32.cu",
         "gemm_f32_split.cu",
         "sampling.cu",
+        "sampling_filters.cu",
     ],
     "gemm": ["gemm_bf16.cu", "gemm_chain.cu", "gemm_bf16_pair.cu"],
     "recurrent": ["recurrent.cu", "scan_blocks.cu"],

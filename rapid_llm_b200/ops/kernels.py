@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
+import numpy as np
 import torch
 
 from .build import attention_library, load_library
@@ -148,6 +149,8 @@ def core() -> ctypes.CDLL:
             c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p,
             c_int, c_void_p,
         ]
+        lib.rl_copy_pages.argtypes = [c_void_p, c_void_p, c_int, c_int, c_longlong, c_longlong, c_int, c_void_p]
+        lib.rl_copy_pages_launches.argtypes = [c_int]
         lib.rl_embedding_sum.argtypes = [
             c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
             c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_int, c_float,
@@ -160,10 +163,14 @@ def core() -> ctypes.CDLL:
             c_int, c_void_p, c_int, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p,
             c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
         ]
+        lib.rl_sample_filtered.argtypes = [
+            c_int, c_void_p, c_int, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+            c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+        ]
         for name in (
-            "rl_embedding", "rl_embedding_sum", "rl_scatter_rows", "rl_add_rmsnorm", "rl_silu_mul", "rl_to_float", "rl_clamped_glu",
+            "rl_sample_filtered", "rl_sample_filtered_max_vocab", "rl_embedding", "rl_embedding_sum", "rl_scatter_rows", "rl_add_rmsnorm", "rl_silu_mul", "rl_to_float", "rl_clamped_glu",
             "rl_rope_unit_write", "rl_layernorm", "rl_row_norm_rope_write", "rl_sigmoid_gate", "rl_relu_squared",
-            "rl_qk_norm_rope_write", "rl_attention_generic", "rl_attention_shared_f32", "rl_gemm_f32", "rl_sample",
+            "rl_qk_norm_rope_write", "rl_attention_generic", "rl_attention_shared_f32", "rl_copy_pages", "rl_copy_pages_launches", "rl_gemm_f32", "rl_sample",
         ):
             getattr(lib, name).restype = c_int
         _SIGNATURES_SET = True
@@ -235,6 +242,36 @@ def scatter_rows(table: torch.Tensor, slots: torch.Tensor, rows: torch.Tensor, f
         "scatter_rows",
     )
     return table
+
+
+def copy_pages(pages: torch.Tensor, pairs) -> torch.Tensor:
+    """``pages[:, target] = pages[:, source]`` for every ``(source, target)`` of ``pairs``, in place: cache pages
+    ``[layers, pages, *page]`` (or per-request states, a layer at a time), of any type.
+
+    ``pairs`` is on the host (a sequence of pairs or an integer array ``[n, 2]``); it is read before the call returns.
+    No target may be named twice or be a source too: the copies run side by side, in no order."""
+    _need_cuda(pages)
+    _contig("pages", pages)
+    if pages.dim() < 2:
+        raise KernelError("copy_pages: pages must be [layers, pages, *page]")
+    pairs = np.asarray(pairs)
+    if pairs.size == 0:
+        return pages
+    if pairs.dtype.kind not in "iu" or pairs.ndim != 2 or pairs.shape[1] != 2:
+        raise KernelError("copy_pages: pairs must be integers [n, 2]")
+    sources, targets = pairs[:, 0].tolist(), pairs[:, 1].tolist()
+    known = pages.shape[1]
+    if min(sources) < 0 or min(targets) < 0 or max(sources) >= known or max(targets) >= known:
+        raise KernelError(f"copy_pages: a pair names a page outside the {known} there are")
+    written = set(targets)
+    if len(written) != len(targets) or not written.isdisjoint(sources):
+        raise KernelError("copy_pages: a page is written twice, or both read and written")
+    listed = np.ascontiguousarray(pairs, dtype=np.int32)
+    size = pages.element_size()
+    _check(core().rl_copy_pages(_ptr(pages), listed.ctypes.data, len(targets), pages.shape[0], pages.stride(0) * size,
+                                pages.stride(1) * size, int(PDL), _stream()), "copy_pages")
+    LAUNCHES.count += core().rl_copy_pages_launches(len(targets)) - 1
+    return pages
 
 
 def add_rmsnorm(
@@ -1206,12 +1243,23 @@ def sample(
     counters: torch.Tensor | None = None,
     seen_tokens: torch.Tensor | None = None,
     seen_offsets: torch.Tensor | None = None,
+    top_k: torch.Tensor | None = None,
+    min_p: torch.Tensor | None = None,
+    uniforms: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """One token per row of ``logits`` into ``out`` (int32); no ``temperature`` = greedy."""
-    _need_cuda(logits, out, temperature, top_p, penalty, seeds, counters, seen_tokens, seen_offsets)
+    """One token per row of ``logits`` into ``out`` (int32); no ``temperature`` = greedy.
+
+    With ``top_k`` (int32; 0 = all), ``min_p`` or ``uniforms`` (float32 in [0, 1): the draws, in place of ``seeds`` and
+    ``counters``) given, a row keeps its ``top_k`` largest logits (of equal ones those of lowest index), of those what has
+    at most ``top_p`` of their mass strictly above it, and of those what has at least ``min_p`` of the largest
+    probability; the draw is the first index whose running kept mass exceeds ``u`` of all kept mass.  Masses are exact to 2^-43 of the
+    largest weight.  A row with ``temperature`` 0 takes the first maximum.  Every array has one entry a row."""
+    _need_cuda(logits, out, temperature, top_p, penalty, seeds, counters, seen_tokens, seen_offsets, top_k, min_p, uniforms)
     _expect("out", out, torch.int32)
-    for name, tensor in (("temperature", temperature), ("top_p", top_p), ("penalty", penalty)):
+    for name, tensor in (("temperature", temperature), ("top_p", top_p), ("penalty", penalty), ("min_p", min_p), ("uniforms", uniforms)):
         _expect(name, tensor, torch.float32)
+    if top_k is not None or min_p is not None or uniforms is not None:
+        return _sample_filtered(logits, out, temperature, top_k, top_p, min_p, penalty, uniforms, seeds, counters, seen_tokens, seen_offsets)
     _expect("seeds", seeds, torch.int64), _expect("counters", counters, torch.int32)
     _expect("seen_tokens", seen_tokens, torch.int32), _expect("seen_offsets", seen_offsets, torch.int32)
     if logits.dim() != 2 or logits.stride(1) != 1 or out.numel() != logits.shape[0]:
@@ -1221,6 +1269,37 @@ def sample(
             dtype_tag(logits.dtype), _ptr(logits), logits.shape[0], logits.shape[1], logits.stride(0),
             _ptr(temperature), _ptr(top_p), _ptr(penalty), _ptr(seeds), _ptr(counters),
             _ptr(seen_tokens), _ptr(seen_offsets), _ptr(out), int(PDL), _stream(),
+        ),
+        f"sample(vocab={logits.shape[1]})",
+    )
+    return out
+
+
+def _sample_filtered(logits, out, temperature, top_k, top_p, min_p, penalty, uniforms, seeds, counters, seen_tokens, seen_offsets):
+    rows = logits.shape[0]
+    if logits.dim() != 2 or logits.stride(1) != 1 or out.numel() != rows:
+        raise KernelError("sample: logits must be [rows, vocab] with contiguous rows and out [rows]")
+    if rows == 0:
+        return out
+    if logits.shape[1] < 1 or logits.shape[1] > core().rl_sample_filtered_max_vocab():
+        raise KernelError(f"sample: rows of {logits.shape[1]} logits are not taken with top_k, min_p or given draws "
+                          f"(at most {core().rl_sample_filtered_max_vocab()})")
+    _expect("top_k", top_k, torch.int32), _expect("seeds", seeds, torch.int64), _expect("counters", counters, torch.int32)
+    _expect("seen_tokens", seen_tokens, torch.int32), _expect("seen_offsets", seen_offsets, torch.int32)
+    for name, tensor in (("out", out), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p),
+                         ("penalty", penalty), ("uniforms", uniforms), ("seeds", seeds), ("counters", counters)):
+        _contig(name, tensor)
+        if tensor is not None and tensor.numel() != rows:
+            raise KernelError(f"sample: {name} must hold one entry per row")
+    if temperature is not None and uniforms is None and (seeds is None or counters is None):
+        raise KernelError("sample: draws need uniforms, or seeds and counters")
+    if (seen_tokens is None) != (seen_offsets is None) or (seen_offsets is not None and seen_offsets.numel() != rows + 1):
+        raise KernelError("sample: the tokens a penalty looks at come with their [rows + 1] offsets")
+    _check(
+        core().rl_sample_filtered(
+            dtype_tag(logits.dtype), _ptr(logits), rows, logits.shape[1], logits.stride(0), _ptr(temperature), _ptr(top_k),
+            _ptr(top_p), _ptr(min_p), _ptr(penalty), _ptr(uniforms), _ptr(seeds), _ptr(counters), _ptr(seen_tokens),
+            _ptr(seen_offsets), _ptr(out), int(PDL), _stream(),
         ),
         f"sample(vocab={logits.shape[1]})",
     )
