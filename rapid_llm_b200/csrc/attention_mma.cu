@@ -608,6 +608,7 @@ int launch_attention(const AttentionArgs& args, int n_items, bool pdl, cudaStrea
 #include "attention_decode_tc.cuh"
 #include "attention_prefill_tc.cuh"
 #include "attention_plane_tc.cuh"
+#include "attention_shared_tc.cuh"
 
 namespace rl {
 namespace RL_ATTENTION_NS {
@@ -682,10 +683,10 @@ static int decode_tc_sm_count() {
   return sms;
 }
 
-template <int kRows, int kStages, bool kDressed>
+template <int kRows, int kStages, bool kDressed, bool kListed = false>
 static int launch_decode_tc_as(const CUtensorMap& map, const DecodeTcArgs& t, int n_items, bool pdl,
                                    cudaStream_t stream, std::atomic<unsigned long long>* configured) {
-  auto kernel = attention_decode_tc_kernel<kRows, kStages, kDressed>;
+  auto kernel = attention_decode_tc_kernel<kRows, kStages, kDressed, kListed>;
   constexpr int kTcSmemBytes = tc_smem_bytes(kStages);
   const cudaError_t allowed = allow_shared(kernel, kTcSmemBytes, *configured, true);      // up to 16 key ranges of a tile
   if (allowed != cudaSuccess) return static_cast<int>(allowed);
@@ -760,6 +761,66 @@ static int launch_decode_tc(const AttentionArgs& a, int n_items, int max_rows, b
   if (max_rows <= 4) return launch_decode_tc_rows<4>(map, t, n_items, pdl, stream, g_decode_tc_configured[2], rings);
   if (max_rows <= 8) return launch_decode_tc_rows<8>(map, t, n_items, pdl, stream, g_decode_tc_configured[3], rings);
   return launch_decode_tc_rows<16>(map, t, n_items, pdl, stream, g_decode_tc_configured[4], rings);
+}
+
+static std::atomic<unsigned long long> g_listed_tc_configured[5][2][2];   // per row-count, ring-depth and sloped instantiation
+
+template <int kRows>
+static int launch_listed_rows_as(const CUtensorMap& map, const DecodeTcArgs& t, int n_items, bool pdl, cudaStream_t stream,
+                                 std::atomic<unsigned long long> (*configured)[2]) {
+  const bool shallow = static_cast<long long>(n_items) * t.hkv > decode_tc_sm_count();
+  if (t.slopes != nullptr)
+    return shallow ? launch_decode_tc_as<kRows, 1, true, true>(map, t, n_items, pdl, stream, &configured[1][1])
+                   : launch_decode_tc_as<kRows, kTcMaxStages, true, true>(map, t, n_items, pdl, stream, &configured[0][1]);
+  return shallow ? launch_decode_tc_as<kRows, 1, false, true>(map, t, n_items, pdl, stream, &configured[1][0])
+                 : launch_decode_tc_as<kRows, kTcMaxStages, false, true>(map, t, n_items, pdl, stream, &configured[0][0]);
+}
+
+// Listed items of up to 16 packed rows on the tcgen05 decode tiles.
+static int launch_listed_rows(const AttentionArgs& a, int n_items, int most_rows, bool early, bool pdl, cudaStream_t stream) {
+  CUtensorMap map;
+  const long long rows = static_cast<long long>(a.num_pages) * 2 * a.hkv * a.page_size;
+  int status = make_map(&map, a.cache, rows, kD, a.page_size < kTcKeys ? a.page_size : kTcKeys);
+  if (status != 0) return status;
+  DecodeTcArgs t = {};
+  t.q = a.q; t.part_out = a.part_out; t.part_lse = a.part_lse; t.items = a.items; t.entry_slot = a.entry_slot;
+  t.block_table = a.block_table; t.hq = a.hq; t.hkv = a.hkv; t.page_size = a.page_size; t.num_pages = a.num_pages;
+  t.max_pages = a.max_pages; t.slots = a.slots; t.splits = 1; t.scale_log2 = a.scale_log2; t.out_stride = a.hq * kTcD;
+  t.slopes = a.slopes; t.fault = a.fault; t.members = a.members; t.positions = a.positions; t.part_first = a.part_first;
+  t.early = early ? 1 : 0;
+  if (most_rows <= 1) return launch_listed_rows_as<1>(map, t, n_items, pdl, stream, g_listed_tc_configured[0]);
+  if (most_rows <= 2) return launch_listed_rows_as<2>(map, t, n_items, pdl, stream, g_listed_tc_configured[1]);
+  if (most_rows <= 4) return launch_listed_rows_as<4>(map, t, n_items, pdl, stream, g_listed_tc_configured[2]);
+  if (most_rows <= 8) return launch_listed_rows_as<8>(map, t, n_items, pdl, stream, g_listed_tc_configured[3]);
+  return launch_listed_rows_as<16>(map, t, n_items, pdl, stream, g_listed_tc_configured[4]);
+}
+
+static std::atomic<unsigned long long> g_shared_tc_configured[2][2];
+
+// Listed items of up to 128 or 256 packed rows.
+template <bool kTwoTiles, bool kSloped>
+static int launch_shared_tc_as(const CUtensorMap& map, const SharedTcArgs& t, int n_items, bool pdl, cudaStream_t stream) {
+  auto kernel = attention_shared_tc_kernel<kTwoTiles, kSloped>;
+  const cudaError_t e = allow_shared(kernel, sh_smem_bytes(kTwoTiles), g_shared_tc_configured[kTwoTiles][kSloped]);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  return launch_kernel(kernel, dim3(t.hkv, n_items), dim3(kShThreads), sh_smem_bytes(kTwoTiles), stream, pdl, map, t);
+}
+
+static int launch_shared_tc(const AttentionArgs& a, int n_items, int tile_rows, bool pdl, cudaStream_t stream) {
+  CUtensorMap map;
+  const long long rows = static_cast<long long>(a.num_pages) * 2 * a.hkv * a.page_size;
+  int status = make_map(&map, a.cache, rows, kD, a.page_size < kShKeys ? a.page_size : kShKeys);
+  if (status != 0) return status;
+  SharedTcArgs t = {};
+  t.q = a.q; t.part_out = a.part_out; t.part_lse = a.part_lse; t.items = a.items; t.entry_slot = a.entry_slot;
+  t.block_table = a.block_table; t.members = a.members; t.positions = a.positions; t.part_first = a.part_first;
+  t.hq = a.hq; t.hkv = a.hkv; t.page_size = a.page_size; t.num_pages = a.num_pages; t.max_pages = a.max_pages; t.slots = a.slots;
+  t.scale_log2 = a.scale_log2; t.slopes = a.slopes; t.fault = a.fault;
+  if (tile_rows == 2 * kShTileRows)
+    return a.slopes != nullptr ? launch_shared_tc_as<true, true>(map, t, n_items, pdl, stream)
+                               : launch_shared_tc_as<true, false>(map, t, n_items, pdl, stream);
+  return a.slopes != nullptr ? launch_shared_tc_as<false, true>(map, t, n_items, pdl, stream)
+                             : launch_shared_tc_as<false, false>(map, t, n_items, pdl, stream);
 }
 
 }  // namespace RL_ATTENTION_NS
@@ -909,8 +970,10 @@ int rl_attention_mma(const void* q, const void* cache, void* out, float* part_ou
   return status;
 }
 
-// Attention over shared prefixes (attention_shared.h): tile_items of up to tile_rows packed rows, row_items of up to 16,
-// [n, 8] int32 each, then the join.  tile_rows: 64 = the mma.sync tiles.
+// Attention over shared prefixes (attention_shared.h): tile_items of up to tile_rows packed rows, row_items of up to 16 (most_rows: the
+// most any has), [n, 8] int32 each, then the join.  tile_rows: 64 = the mma.sync tiles for both lists, 128 or 256 = the
+// tcgen05 tiles for both (head size 128, pages they take).  The kernels of one call follow each other as dependent launches: the
+// second starts while the first still runs (both read the queries and write parts of their own), the join waits for both.
 int rl_attention_shared(const void* q, const void* cache, void* out, float* part_out, float* part_lse, const int* tile_items,
                         int n_tile_items, int tile_rows, const int* row_items, int n_row_items, int most_rows,
                         const int* members, const int* positions, const int* part_first, const int* entry_slot,
@@ -919,7 +982,9 @@ int rl_attention_shared(const void* q, const void* cache, void* out, float* part
                         const void* gate, int gate_stride, int* fault, int pdl, cudaStream_t stream) {
   if (tokens == 0) return 0;
   if (head_dim != attn::kD || hkv <= 0 || hq % hkv != 0 || page_size <= 0 || hkv > 65535 || n_tile_items < 0 || n_row_items < 0 ||
-      n_tile_items > 65535 || n_row_items > 65535 || tile_rows != 64 || out_stride < hq * head_dim || out_stride % 8 != 0 ||
+      n_tile_items > 65535 || n_row_items > 65535 || (tile_rows != 64 && tile_rows != 128 && tile_rows != 256) ||
+      (tile_rows != 64 && !attn::decode_tc_supported(page_size)) ||
+      static_cast<long long>(num_pages) * 2 * hkv * page_size > 0x7fffffffll || out_stride < hq * head_dim || out_stride % 8 != 0 ||
       (reinterpret_cast<uintptr_t>(out) & 15) || (gate != nullptr && gate_stride < hq) ||
       static_cast<long long>(tokens) * hq > 0x7fffffffll)
     return static_cast<int>(cudaErrorInvalidValue);
@@ -938,21 +1003,38 @@ int rl_attention_shared(const void* q, const void* cache, void* out, float* part
   args.members = members; args.positions = positions; args.part_first = part_first;
   args.fault = fault;
   int status = 0;
-  if (n_tile_items > 0) {
-    args.items = tile_items;
-    status = slopes != nullptr ? attn::launch_attention_as<4, 1, 2, false, true, true>(args, n_tile_items, pdl != 0, stream)
-                               : attn::launch_attention_as<4, 1, 2, false, false, true>(args, n_tile_items, pdl != 0, stream);
-    if (status != 0) return status;
+  if constexpr (attn::kD == attn::kTcD) {
+    if (tile_rows != 64) {
+      if (n_tile_items > 0) {
+        args.items = tile_items;
+        status = attn::launch_shared_tc(args, n_tile_items, tile_rows, pdl != 0, stream);
+        if (status != 0) return status;
+      }
+      if (n_row_items > 0) {
+        args.items = row_items;
+        status = attn::launch_listed_rows(args, n_row_items, most_rows, n_tile_items > 0, n_tile_items > 0 || pdl != 0, stream);
+        if (status != 0) return status;
+      }
+    }
   }
-  if (n_row_items > 0) {
-    args.items = row_items;
-    status = slopes != nullptr ? attn::launch_attention_as<1, 4, 3, false, true, true>(args, n_row_items, pdl != 0, stream)
-                               : attn::launch_attention_as<1, 4, 3, false, false, true>(args, n_row_items, pdl != 0, stream);
-    if (status != 0) return status;
+  if (tile_rows == 64) {
+    if (n_tile_items > 0) {
+      args.items = tile_items;
+      status = slopes != nullptr ? attn::launch_attention_as<4, 1, 2, false, true, true>(args, n_tile_items, pdl != 0, stream)
+                                 : attn::launch_attention_as<4, 1, 2, false, false, true>(args, n_tile_items, pdl != 0, stream);
+      if (status != 0) return status;
+    }
+    if (n_row_items > 0) {
+      args.items = row_items;
+      const bool dependent = n_tile_items > 0 || pdl != 0;
+      status = slopes != nullptr ? attn::launch_attention_as<1, 4, 3, false, true, true>(args, n_row_items, dependent, stream)
+                                 : attn::launch_attention_as<1, 4, 3, false, false, true>(args, n_row_items, dependent, stream);
+      if (status != 0) return status;
+    }
   }
   const int rows = tokens * hq;
   return rl::launch_kernel(rl::attention_join_kernel<attn::bf16>, dim3((rows + rl::kJoinWarps - 1) / rl::kJoinWarps),
-                           dim3(rl::kJoinWarps * 32), 0, stream, pdl != 0, part_out, part_lse, part_first,
+                           dim3(rl::kJoinWarps * 32), 0, stream, pdl != 0 || n_tile_items > 0 || n_row_items > 0, part_out, part_lse, part_first,
                            static_cast<attn::bf16*>(out), rows, hq, head_dim, out_stride, sink,
                            static_cast<const attn::bf16*>(gate), gate_stride);
 }

@@ -806,6 +806,7 @@ def attention_mma(
 
 
 SHARED_F32_ROWS = 32      # packed rows of an item of the float32 kernel over shared prefixes
+SHARED_TC_ROWS = (128, 256)   # ... of the tcgen05 kernel: one tile or two
 SHARED_ITEM = 8           # numbers that describe an item
 
 
@@ -853,6 +854,8 @@ def attention_shared(
         raise KernelError("attention: q and out must be [tokens, heads * head_dim] of the cache's dtype")
     if plan["tokens"] != tokens or plan["heads"] != (num_heads // num_kv_heads, num_kv_heads, head_dim) or plan["dtype"] != dtype_tag(q.dtype):
         raise KernelError("attention: the plan was made for another step")
+    if not scale > 0:
+        raise KernelError("attention: the scale must be positive")
     if plan["entries"] != entry_slot.numel() or block_table.dim() != 2:
         raise KernelError("attention: the plan was made for another number of entries")
     out_stride, gate_stride = _attention_out(out, gate, tokens, num_heads, head_dim)

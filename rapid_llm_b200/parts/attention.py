@@ -243,6 +243,7 @@ class SharedItems(StepPlanner):
     def __init__(self, group: int, num_kv_heads: int, head_dim: int, sms: int = DEFAULT_SMS, dtype: torch.dtype = torch.bfloat16) -> None:
         self.group, self.num_kv_heads, self.head_dim, self.sms = int(group), int(num_kv_heads), int(head_dim), int(sms)
         self.wide = dtype == torch.float32
+        self.ctas_per_sm = 2
         self.tag = kernels.dtype_tag(dtype)
         self.key = ("shared_items", self.group, self.num_kv_heads, self.head_dim, self.sms, self.tag)
 
@@ -280,21 +281,29 @@ class SharedItems(StepPlanner):
             work.append((entry, int(shared[entry]), int(starts[entry] + lengths[entry]), int(first_token[entry]), len(its),
                          int(starts[entry]), its))
 
-        tile_rows = kernels.SHARED_F32_ROWS if self.wide else kernels.CHUNK_TILE_ROWS
+        packed_rows = [n * self.group for _, _, _, _, n, _, _ in work]
+        if self.wide:
+            tile_rows = kernels.SHARED_F32_ROWS
+        elif not kernels.attention_tc_takes(self.head_dim, shape.page_size):
+            tile_rows = kernels.CHUNK_TILE_ROWS
+        else:
+            tile_rows = kernels.SHARED_TC_ROWS[max(packed_rows) > kernels.SHARED_TC_ROWS[0]]
 
-        def rows_of(rows: int) -> int:
-            return tile_rows if self.wide or rows > kernels.DECODE_TILE_ROWS else kernels.DECODE_TILE_ROWS
+        def height_of(rows: int) -> int:
+            if not self.wide and rows <= kernels.DECODE_TILE_ROWS:
+                return kernels.DECODE_TILE_ROWS
+            tiles = -(-rows // tile_rows)
+            return min(tile_rows, -(-(-(-rows // tiles)) // 32) * 32)       # even tiles of whole warps
 
-        units = sum(-(-(end - first) // block) * -(-n * self.group // rows_of(n * self.group))
-                    for _, first, end, _, n, _, _ in work) * self.num_kv_heads
-        ctas = 2 * self.sms
-        per_item = max(1, -(-units // ctas))                    # blocks of keys an item takes
+        units = sum(-(-(end - first) // block) * -(-rows // height_of(rows))
+                    for (_, first, end, _, _, _, _), rows in zip(work, packed_rows)) * self.num_kv_heads
+        per_item = max(1, -(-units // (self.ctas_per_sm * self.sms)))       # blocks of keys an item takes
         parts = np.zeros(tokens, dtype=np.int64)                # of each token so far: a group's items come before its entries'
         tiles, rows, most = [], [], 0
         for entry, first, end, member, n, fresh, its in work:
             packed = n * self.group
-            height = rows_of(packed)
-            bucket = tiles if height == tile_rows else rows
+            height = height_of(packed)
+            bucket = rows if not self.wide and packed <= kernels.DECODE_TILE_ROWS else tiles
             if bucket is rows:
                 most = max(most, min(height, packed))
             ranges = max(1, -(-(end - first) // (per_item * block)))

@@ -131,3 +131,153 @@ def test_equals_each_requests_own_attention(shape, dtype, layout):
     }[layout]
     step = Step(prefix, requests, dtype=dtype, seed=len(requests), **shape)
     check(step.run(), step.want(), dtype, shape["dim"])
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256, 24])
+@pytest.mark.parametrize("members,group", [(5, 4), (30, 4), (33, 4), (64, 4), (52, 5), (70, 8), (7, 16)])
+def test_tiles_of_every_height_and_page(page, members, group):
+    """128 wide heads: one tile, two tiles, several items of two; prefixes that end inside a block of 128 keys, and one beyond."""
+    for prefix in (page * 3, max(page, 1100 // page * page)):
+        step = Step([prefix], [(0, 1 + 13 * i % 150, 1) for i in range(members)], heads=2 * group, kv_heads=2, dim=128, page=page,
+                    dtype=torch.bfloat16, seed=members + page)
+        check(step.run(), step.want(), torch.bfloat16, 128)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_what_lies_behind_a_request_is_not_seen(dtype, dim):
+    """NaN in every place of the cache that no request holds, the places behind a request's last key in its own page among them."""
+    for members in (3, 40):
+        step = Step([176, 32], [(0, 1 + 7 * i % 40, 1) for i in range(members)] + [(1, 3, 2), (-1, 130, 1)], heads=8, kv_heads=2, dim=dim,
+                    page=16, dtype=dtype, seed=3)
+        held = torch.zeros(step.cache.shape[0], step.page, dtype=torch.bool, device=DEV)
+        for e, (start, new) in enumerate(zip(step.starts, step.new)):
+            at = np.arange(start + new)
+            held[torch.from_numpy(step.table[step.slots[e], at // step.page].astype(np.int64)).to(DEV), torch.from_numpy(at % step.page).to(DEV)] = True
+        step.cache.permute(0, 3, 1, 2, 4)[~held] = float("nan")
+        check(step.run(), step.want(), dtype, dim)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("members", [2, 12, 40])
+def test_sink_gate_slopes_and_wider_rows(dtype, members, dim):
+    step = Step([320], [(0, 1 + 11 * i % 90, 1 + i % 2) for i in range(members)] + [(-1, 40, 1)], heads=12, kv_heads=3, dim=dim, page=16,
+                dtype=dtype, seed=members)
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    tokens = len(step.positions)
+    sink = torch.randn((12,), generator=gen, device=DEV) * 3
+    sink[1] = -float("inf")
+    slopes = torch.rand((12,), generator=gen, device=DEV) * 0.2
+    slopes[0] = 0.0
+    wide_gate = torch.randn((tokens, 40), generator=gen, device=DEV).to(dtype)
+    gate = wide_gate[:, 16:28]
+    wide_out = torch.full((tokens, 12 * dim + 32), 7.0, dtype=dtype, device=DEV)
+    out = wide_out[:, 16 : 16 + 12 * dim]
+    for options in ({"sink": sink}, {"slopes": slopes}, {"gate": gate}, {"sink": sink, "slopes": slopes, "gate": gate}):
+        got = step.run(out=out, **options)
+        want, size, largest = step.want(**options)
+        check(got, (want, size, largest + float(slopes.max()) * 420), dtype, dim)
+    assert bool((wide_out[:, :16] == 7.0).all()) and bool((wide_out[:, 16 + 12 * dim :] == 7.0).all())
+
+
+def test_the_largest_head_and_wide_groups():
+    for dtype, dim, heads, kv in ((torch.float32, 256, 4, 2), (torch.float32, 16, 40, 1), (torch.bfloat16, 128, 20, 1), (torch.bfloat16, 128, 150, 1)):
+        step = Step([400], [(0, 1 + 3 * i, 1) for i in range(9)], heads=heads, kv_heads=kv, dim=dim, page=16, dtype=dtype, seed=heads)
+        check(step.run(), step.want(), dtype, dim)
+
+
+def test_equals_the_unshared_kernel_on_a_captured_step():
+    """The captured call on another stream, replayed with the scratch and the result spoiled in between, new queries each time."""
+    step = Step([1024], [(0, 1 + 9 * i, 1) for i in range(20)], heads=16, kv_heads=4, dim=128, page=16, dtype=torch.bfloat16)
+    plan = step.device_plan()
+    rows = step.planner.part_rows(plan)
+    part_out, part_lse = torch.empty((rows, 128), device=DEV), torch.empty((rows,), device=DEV)
+    to = lambda values: torch.from_numpy(np.ascontiguousarray(np.asarray(values, dtype=np.int32))).to(DEV)
+    out = torch.empty_like(step.q)
+    fixed = dict(plan=plan, part_out=part_out, part_lse=part_lse, positions=to(step.positions), cu_seqlens=to(np.arange(21)),
+                 entry_start=to(step.starts), entry_slot=to(step.slots), block_table=to(step.table), num_heads=16, num_kv_heads=4,
+                 head_dim=128, scale=step.scale, fault=step.fault)
+    kernels.attention_shared(step.q, step.cache, out, **fixed)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    previous, kernels.PDL = kernels.PDL, True
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(3):                     # layers one after the other on the same scratch
+                kernels.attention_shared(step.q, step.cache, out, **fixed)
+    finally:
+        kernels.PDL = previous
+    for seed in range(3):
+        step.q.copy_(torch.randn(step.q.shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV))
+        part_out.fill_(float("nan")), part_lse.fill_(float("nan")), out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, step.want(), torch.bfloat16, 128)
+    assert int(step.fault.item()) == 0
+
+
+def test_the_same_bits_every_time():
+    for dtype, dim in ((torch.float32, 80), (torch.bfloat16, 64), (torch.bfloat16, 128)):
+        step = Step([900 // 16 * 16], [(0, 1 + 9 * i, 1) for i in range(40)], heads=16, kv_heads=4, dim=dim, page=16, dtype=dtype)
+        first = step.run()
+        for _ in range(5):
+            assert torch.equal(step.run(), first)
+
+
+def test_a_page_or_slot_outside_the_pool_is_reported():
+    """Indices that the kernels look at before they use them (no access is made through a bad one)."""
+    for dtype, dim in ((torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 128)):
+        for spoil, word in ((lambda s: s.table.__setitem__((s.slots[0], 2), 10_000), 2), (lambda s: s.table.__setitem__((s.slots[1], 12), -3), 2),
+                            (lambda s: s.slots.__setitem__(1, 77), 8)):
+            step = Step([160], [(0, 40, 1) for _ in range(8)], heads=8, kv_heads=2, dim=dim, page=16, dtype=dtype)
+            step.slots = step.slots.copy()
+            spoil(step)
+            with pytest.raises(AssertionError):
+                step.run()
+            assert int(step.fault.item()) & word
+
+
+def _call(step, **changed):
+    plan = step.device_plan()
+    rows = step.planner.part_rows(plan)
+    to = lambda values: torch.from_numpy(np.ascontiguousarray(np.asarray(values, dtype=np.int32))).to(DEV)
+    arguments = dict(q=step.q, cache=step.cache, out=torch.empty_like(step.q), plan=plan, part_out=torch.empty((rows, step.dim), device=DEV),
+                     part_lse=torch.empty((rows,), device=DEV), positions=to(step.positions), cu_seqlens=to(np.arange(len(step.new) + 1)),
+                     entry_start=to(step.starts), entry_slot=to(step.slots), block_table=to(step.table), num_heads=step.heads,
+                     num_kv_heads=step.kv_heads, head_dim=step.dim, scale=step.scale, fault=step.fault)
+    arguments.update({k: v(arguments) for k, v in changed.items()})
+    return kernels.attention_shared(arguments.pop("q"), arguments.pop("cache"), arguments.pop("out"), **arguments)
+
+
+REFUSED = [
+    dict(q=lambda a: a["q"][:1]), dict(q=lambda a: a["q"].float()), dict(q=lambda a: a["q"].half()), dict(cache=lambda a: a["cache"][:, :1]), dict(cache=lambda a: a["cache"].float()),
+    dict(part_out=lambda a: a["part_out"][1:]), dict(part_lse=lambda a: None), dict(part_out=lambda a: a["part_out"].bfloat16()),
+    dict(positions=lambda a: a["positions"].long()), dict(positions=lambda a: a["positions"][:2]), dict(entry_slot=lambda a: a["entry_slot"][:2]),
+    dict(scale=lambda a: 0.0), dict(scale=lambda a: float("nan")), dict(num_heads=lambda a: 7), dict(head_dim=lambda a: 32),
+    dict(out=lambda a: a["out"].float()), dict(sink=lambda a: torch.zeros(3, device=DEV)), dict(gate=lambda a: torch.zeros((3, 2), device=DEV)),
+    dict(fault=lambda a: a["fault"].cpu()), dict(plan=lambda a: {**a["plan"], "dtype": 0}), dict(plan=lambda a: {**a["plan"], "tokens": 9}),
+    dict(plan=lambda a: {**a["plan"], "members": a["plan"]["members"].cpu()}), dict(block_table=lambda a: a["block_table"].T),
+]
+
+
+@pytest.mark.parametrize("changed", REFUSED, ids=lambda c: next(iter(c)))
+def test_refused(changed):
+    step = Step([64], [(0, 3, 1), (0, 5, 1), (0, 1, 1)], heads=8, kv_heads=2, dim=64, page=16, dtype=torch.bfloat16)
+    with pytest.raises(kernels.KernelError):
+        _call(step, **changed)
+
+
+@pytest.mark.parametrize("own", [129, 500, 1024, 1500])
+def test_long_keys_of_their_own_walked_by_one_item(own):
+    """Many requests behind a long prefix: an item walks all of a request's own keys, in several blocks, with the ring of one
+    tile a multiprocessor shares; and values behind the last key that are NaN."""
+    step = Step([16000], [(0, max(1, own - 17 * i % own), 1) for i in range(64)], heads=20, kv_heads=4, dim=128, page=16, dtype=torch.bfloat16, seed=own)
+    held = torch.zeros(step.cache.shape[0], step.page, dtype=torch.bool, device=DEV)
+    for e, (start, new) in enumerate(zip(step.starts, step.new)):
+        at = np.arange(start + new)
+        held[torch.from_numpy(step.table[step.slots[e], at // step.page].astype(np.int64)).to(DEV), torch.from_numpy(at % step.page).to(DEV)] = True
+    step.cache.permute(0, 3, 1, 2, 4)[~held] = float("nan")
+    want = step.want()
+    for _ in range(4):
+        check(step.run(), want, torch.bfloat16, 128)
