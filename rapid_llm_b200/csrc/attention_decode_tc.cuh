@@ -82,11 +82,6 @@ struct DecodeTcArgs {
   const float* sink;        // [hq] float32 or null: exp(sink[head]) joins every row's denominator once
   const float* slopes;      // [hq] float32 or null: slopes[head] * (query position - key position) is taken off every score
   int* fault;
-  // Listed items (attention_shared.h)
-  const int* members;
-  const int* positions;
-  const int* part_first;
-  int early;                // the kernel before is the same operator's, which passed its own wait before this one could start
 };
 
 // Largest value over the warp's lanes in one instruction.
@@ -96,23 +91,10 @@ __device__ __forceinline__ float warp_max_redux(float v) {
   return r;
 }
 
-// Rows `first` .. 127 of a tile of 128 keys (two halves of 128-byte rows) become zeros, by one warp, for the tensor cores to see.
-__device__ __forceinline__ void clear_rows(uint32_t tile, int first, int lane) {
-  for (int i = first * 16 + lane; i < kTcKeys * 16; i += 32) {
-    const uint32_t at = tile + ((i >> 3) & 1) * kTcHalfBytes + (i >> 4) * 128 + (i & 7) * 16;
-    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0) : "memory");
-  }
-  fence_async_smem();
-  __syncwarp();
-}
-
 // kRows: how many of the 16 columns of the products carry query rows (a power of two); the
 // per-row work of the softmax threads is unrolled over exactly these.  kDressed: scores know slopes, the row's last step a sink, a
 // gate and an output whose rows are some columns of wider ones (the plain form keeps its registers and its short tail).
-// kListed: an item names its rows' tokens and its key range itself and leaves a part of each row's result (attention_shared.h).
-// Beyond the keys' end it clears the values that came along in the last block: a weight of zero times what may lie there (a
-// NaN) would not be zero.
-template <int kRows, int kTcStages, bool kDressed, bool kListed = false>
+template <int kRows, int kTcStages, bool kDressed>
 __global__ void __launch_bounds__(kTcThreads, kTcStages == 1 ? 2 : 1)
 attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const DecodeTcArgs args) {
   static_assert(kRows >= 1 && kRows <= kTcRows && (kRows & (kRows - 1)) == 0, "rows: a power of two up to 16");
@@ -139,40 +121,28 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
   auto p_tile = [&](int team, int b) { return q_tile + (1 + team * 2 + b) * kTcOperandBytes; };
 
   // ---- the item ------------------------------------------------------------------------
-  const int* item = args.items + (static_cast<size_t>(blockIdx.z) * gridDim.x + blockIdx.x) * (kListed ? kListedInts : 4);
-  const int entry = item[0];
-  const int row0 = kListed ? item[kListedRow0] : item[1], split = kListed ? item[kListedPart] : item[2];
+  const int* item = args.items + (static_cast<size_t>(blockIdx.z) * gridDim.x + blockIdx.x) * 4;
+  const int entry = item[0], row0 = item[1], split = item[2];
   const int kv_head = blockIdx.y;
   const int group = args.hq / args.hkv;
-  const int tok_begin = kListed ? 0 : args.cu_seqlens[entry];
-  const int n_rows_entry = kListed ? row0 + item[kListedRows] : (args.cu_seqlens[entry + 1] - tok_begin) * group;
+  const int tok_begin = args.cu_seqlens[entry];
+  const int n_rows_entry = (args.cu_seqlens[entry + 1] - tok_begin) * group;
   const int n_rows = min(kRows, n_rows_entry - row0);
-  if constexpr (kListed) {
-    if (n_rows <= 0) {                              // a place of the list that holds no item
-      pdl_wait();
-      return;
-    }
-  }
-  const int start = kListed ? item[kListedFresh] : args.entry_start[entry];
+  const int start = args.entry_start[entry];
   const int slot = args.entry_slot[entry];
-  const int* members = kListed ? args.members + item[kListedMembers] : nullptr;
-  auto token_at = [&](int token) { return kListed ? members[token] : tok_begin + token; };
   const int last_row = row0 + n_rows - 1;
-  const int min_pos = kListed ? item[kListedFirst] : start + row0 / group;
-  const int max_pos = kListed ? item[kListedEnd] - 1 : start + last_row / group;
-  const bool bad = slot < 0 || slot >= args.slots || start < 0 || n_rows <= 0 || min_pos < 0 ||
+  const int min_pos = start + row0 / group, max_pos = start + last_row / group;
+  const bool bad = slot < 0 || slot >= args.slots || start < 0 || n_rows <= 0 ||
                    max_pos >= args.max_pages * args.page_size;
   if (bad && tid == 0)
     atomicOr(args.fault, (slot < 0 || slot >= args.slots) ? kFaultSlot : kFaultPosition);
   const int hi = bad ? 0 : max_pos + 1;
-  const int lo = kListed ? min_pos : first_visible(min_pos, args.window, args.chunk);
-  // a listed item's blocks start where a box of the copies does
-  const int lo_aligned = kListed ? lo - lo % min(args.page_size, kTcKeys) : lo & ~(kTcKeys - 1);
+  const int lo = first_visible(min_pos, args.window, args.chunk);
+  const int lo_aligned = lo & ~(kTcKeys - 1);
   const int span = max(hi - lo_aligned, 0);
   const int per_split = ((span + args.splits - 1) / args.splits + kTcKeys - 1) / kTcKeys * kTcKeys;
-  const int k_begin = kListed ? lo_aligned : lo_aligned + split * per_split;
-  const int k_end = kListed ? hi : min(hi, k_begin + per_split);
-  const bool early = kListed && args.early;         // queries are there; the wait comes last
+  const int k_begin = lo_aligned + split * per_split;
+  const int k_end = min(hi, k_begin + per_split);
   const int n_blocks = k_end > k_begin ? (k_end - k_begin + kTcKeys - 1) / kTcKeys : 0;
   const int* table = args.block_table + static_cast<size_t>(bad ? 0 : slot) * args.max_pages;
 
@@ -202,9 +172,9 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
   }
   if (tid < kTcRows) {
     const int p = row0 + tid;
-    const int pos = tid >= n_rows ? -1 : kListed ? args.positions[members[p / group]] : start + p / group;   // -1: a row that sees no key
+    const int pos = tid < n_rows ? start + p / group : -1;       // -1: a row that sees no key
     row_pos[tid] = pos;
-    row_lo[tid] = kListed ? lo : first_visible(pos, args.window, args.chunk);
+    row_lo[tid] = first_visible(pos, args.window, args.chunk);
   }
   // the page ids of this item's key range (the block table is complete before the step starts)
   const int first_page = k_begin / args.page_size;
@@ -256,7 +226,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
       }
       // keys from `start` on are written by this step's earlier kernels
       if (!waited && kb + kTcKeys > start) {
-        if (!early) pdl_wait();
+        pdl_wait();
         waited = true;
       }
       if (lane == 0) mbar_expect_tx(smem_addr(&fulls[stage]), kTcTileBytes / 2);
@@ -286,13 +256,12 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
       }
       ++issued;
     }
-    if (!waited && !early) pdl_wait();
+    if (!waited) pdl_wait();
     if (lane == 0 && n_blocks > 0 && (!ok || *aborted)) {
       // copies in flight must land before the CTA may exit
-      volatile int go_on = 0;
       for (int s = 0; s < kTcStages; ++s) {
         const int fills = (issued - s + kTcStages - 1) / kTcStages;
-        if (fills > 0) mbar_wait(smem_addr(&fulls[s]), (fills - 1) & 1, kListed ? &go_on : aborted, args.fault);
+        if (fills > 0) mbar_wait(smem_addr(&fulls[s]), (fills - 1) & 1, aborted, args.fault);
       }
     }
   } else if (warp == kTcIssuerWarp) {
@@ -334,10 +303,6 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
         if (next_pv < next_s) {
           const int stage = next_pv % kTcStages, team = next_pv & 1, buf = (next_pv >> 1) & 1;
           if (there(&p_ready[team][buf], next_pv >> 2) && there(&full_v[stage], next_pv / kTcStages)) {
-            if constexpr (kListed) {
-              // (this warp waits for every block in turn, so the phase it saw is the block's own)
-              if (next_pv == blocks - 1 && k_begin + blocks * kTcKeys > k_end) clear_rows(v_tile(stage), k_end - (k_begin + next_pv * kTcKeys), lane);
-            }
             tc_fence_after();
             const uint64_t values_desc = operand_desc_mn(v_tile(stage), kTcHalfBytes);
             const uint64_t p_desc = operand_desc(p_tile(team, buf));
@@ -390,7 +355,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
     out_acc[n] = 0.0f;
   }
   if (softmax_warp) {
-    if (!early) pdl_wait();                            // queries come from the kernel before
+    pdl_wait();                                        // queries come from the kernel before
     if (team == 0) {
       // Q: 16 rows of 128, as the K-major operand [row][64] x 2 halves with the 128-byte swizzle
       for (int idx = t; idx < kTcRows * 16; idx += 128) {
@@ -399,7 +364,7 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
         if (r < n_rows && !bad) {
           const int p = row0 + r, token = p / group;
           value = *reinterpret_cast<const uint4*>(
-              args.q + (static_cast<size_t>(token_at(token)) * args.hq + kv_head * group + (p - token * group)) * kTcD + c * 8);
+              args.q + (static_cast<size_t>(tok_begin + token) * args.hq + kv_head * group + (p - token * group)) * kTcD + c * 8);
         }
         const uint32_t dst = q_tile + (c >> 3) * (kTcRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(value.x), "r"(value.y), "r"(value.z), "r"(value.w) : "memory");
@@ -530,12 +495,6 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
       float inv = total > 0.0f ? 1.0f / total : 0.0f;
       const float lse = total > 0.0f ? m + log2f(total) : -INFINITY;
       const int p = row0 + n, token = p / group, head = kv_head * group + (p - token * group);
-      if constexpr (kListed) {
-        const size_t at = static_cast<size_t>(args.part_first[members[token]] + split) * args.hq + head;
-        args.part_out[at * kTcD + t] = value * inv;
-        if (t == 0) args.part_lse[at] = lse;
-        continue;
-      }
       const size_t row = static_cast<size_t>(tok_begin + token) * args.hq + head;
       if (kDressed && args.sink != nullptr && args.splits == 1) {
         // an unsplit row's denominator takes the sink here; a split one's where its parts meet
@@ -631,7 +590,6 @@ attention_decode_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
     __syncwarp();
     cluster_sync();   // nobody leaves while its shared memory may still be read
   }
-  if (early) pdl_wait();                            // so that what follows this kernel follows the one before it too
 
   tc_fence_before();
   __syncthreads();

@@ -137,7 +137,7 @@ attention_mma_kernel(const AttentionArgs args) {
   bf16* k_smem = q_smem + kTileM * kStride;                            // [kStages][64][kStride]
   bf16* v_smem = kShared ? k_smem : k_smem + kStages * kBlockN * kStride;   // [kStages][64][kStride], or the keys' own
 
-  pdl_trigger();
+  if constexpr (!kListed) pdl_trigger();       // listed items: after the wait below
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wm = warp % kWarpsM, wn = warp / kWarpsM;
   // the kv head is the fast grid dimension: CTAs start in the order of the item list (longest
@@ -185,6 +185,7 @@ attention_mma_kernel(const AttentionArgs args) {
   if constexpr (kListed) {
     if (last_row < row0) {       // a place of the list that holds no item
       pdl_wait();
+      pdl_trigger();
       return;
     }
   }
@@ -306,6 +307,7 @@ attention_mma_kernel(const AttentionArgs args) {
   };
 
   pdl_wait();   // queries and this step's keys come from the kernels before
+  if constexpr (kListed) pdl_trigger();        // what follows need not wait for those kernels again
   load_q();
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
@@ -456,7 +458,7 @@ attention_mma_kernel(const AttentionArgs args) {
 #pragma unroll
         for (int nt = 0; nt < kD / 8; ++nt)
           *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(o_acc[nt][2 * i] * inv, o_acc[nt][2 * i + 1] * inv);
-        if ((lane & 3) == 0) args.part_lse[at] = run_sum[i] > 0.0f ? run_max[i] + log2f(run_sum[i]) : -INFINITY;
+        if ((lane & 3) == 0) args.part_lse[at] = run_sum[i] == 0.0f ? -INFINITY : run_max[i] + log2f(run_sum[i]);
         continue;
       }
       const size_t row = static_cast<size_t>(row_token[i]) * args.hq + row_head[i];
@@ -525,7 +527,7 @@ attention_mma_kernel(const AttentionArgs args) {
       if constexpr (kListed) {
         const size_t at = static_cast<size_t>(args.part_first[members[token]] + split) * args.hq + head;
         args.part_out[at * kD + c] = value * inv;
-        if (c == 0) args.part_lse[at] = total > 0.0f ? m + log2f(total) : -INFINITY;
+        if (c == 0) args.part_lse[at] = total == 0.0f ? -INFINITY : m + log2f(total);
         continue;
       }
       const size_t row = static_cast<size_t>(tok_begin + token) * args.hq + head;
@@ -609,6 +611,7 @@ int launch_attention(const AttentionArgs& args, int n_items, bool pdl, cudaStrea
 #include "attention_prefill_tc.cuh"
 #include "attention_plane_tc.cuh"
 #include "attention_shared_tc.cuh"
+#include "attention_rows.cuh"
 
 namespace rl {
 namespace RL_ATTENTION_NS {
@@ -683,10 +686,10 @@ static int decode_tc_sm_count() {
   return sms;
 }
 
-template <int kRows, int kStages, bool kDressed, bool kListed = false>
+template <int kRows, int kStages, bool kDressed>
 static int launch_decode_tc_as(const CUtensorMap& map, const DecodeTcArgs& t, int n_items, bool pdl,
                                    cudaStream_t stream, std::atomic<unsigned long long>* configured) {
-  auto kernel = attention_decode_tc_kernel<kRows, kStages, kDressed, kListed>;
+  auto kernel = attention_decode_tc_kernel<kRows, kStages, kDressed>;
   constexpr int kTcSmemBytes = tc_smem_bytes(kStages);
   const cudaError_t allowed = allow_shared(kernel, kTcSmemBytes, *configured, true);      // up to 16 key ranges of a tile
   if (allowed != cudaSuccess) return static_cast<int>(allowed);
@@ -763,36 +766,20 @@ static int launch_decode_tc(const AttentionArgs& a, int n_items, int max_rows, b
   return launch_decode_tc_rows<16>(map, t, n_items, pdl, stream, g_decode_tc_configured[4], rings);
 }
 
-static std::atomic<unsigned long long> g_listed_tc_configured[5][2][2];   // per row-count, ring-depth and sloped instantiation
-
-template <int kRows>
-static int launch_listed_rows_as(const CUtensorMap& map, const DecodeTcArgs& t, int n_items, bool pdl, cudaStream_t stream,
-                                 std::atomic<unsigned long long> (*configured)[2]) {
-  const bool shallow = static_cast<long long>(n_items) * t.hkv > decode_tc_sm_count();
-  if (t.slopes != nullptr)
-    return shallow ? launch_decode_tc_as<kRows, 1, true, true>(map, t, n_items, pdl, stream, &configured[1][1])
-                   : launch_decode_tc_as<kRows, kTcMaxStages, true, true>(map, t, n_items, pdl, stream, &configured[0][1]);
-  return shallow ? launch_decode_tc_as<kRows, 1, false, true>(map, t, n_items, pdl, stream, &configured[1][0])
-                 : launch_decode_tc_as<kRows, kTcMaxStages, false, true>(map, t, n_items, pdl, stream, &configured[0][0]);
-}
-
-// Listed items of up to 16 packed rows on the tcgen05 decode tiles.
-static int launch_listed_rows(const AttentionArgs& a, int n_items, int most_rows, bool early, bool pdl, cudaStream_t stream) {
-  CUtensorMap map;
-  const long long rows = static_cast<long long>(a.num_pages) * 2 * a.hkv * a.page_size;
-  int status = make_map(&map, a.cache, rows, kD, a.page_size < kTcKeys ? a.page_size : kTcKeys);
-  if (status != 0) return status;
-  DecodeTcArgs t = {};
-  t.q = a.q; t.part_out = a.part_out; t.part_lse = a.part_lse; t.items = a.items; t.entry_slot = a.entry_slot;
-  t.block_table = a.block_table; t.hq = a.hq; t.hkv = a.hkv; t.page_size = a.page_size; t.num_pages = a.num_pages;
-  t.max_pages = a.max_pages; t.slots = a.slots; t.splits = 1; t.scale_log2 = a.scale_log2; t.out_stride = a.hq * kTcD;
-  t.slopes = a.slopes; t.fault = a.fault; t.members = a.members; t.positions = a.positions; t.part_first = a.part_first;
-  t.early = early ? 1 : 0;
-  if (most_rows <= 1) return launch_listed_rows_as<1>(map, t, n_items, pdl, stream, g_listed_tc_configured[0]);
-  if (most_rows <= 2) return launch_listed_rows_as<2>(map, t, n_items, pdl, stream, g_listed_tc_configured[1]);
-  if (most_rows <= 4) return launch_listed_rows_as<4>(map, t, n_items, pdl, stream, g_listed_tc_configured[2]);
-  if (most_rows <= 8) return launch_listed_rows_as<8>(map, t, n_items, pdl, stream, g_listed_tc_configured[3]);
-  return launch_listed_rows_as<16>(map, t, n_items, pdl, stream, g_listed_tc_configured[4]);
+// Listed items of up to 16 packed rows: from memory straight into the tensor cores' registers (heads of 64 and 128).
+static int launch_rows(const AttentionArgs& a, int n_items, int most_rows, bool early, bool pdl, cudaStream_t stream) {
+  if constexpr (!kRwTakes) {
+    return static_cast<int>(cudaErrorInvalidValue);
+  } else {
+    RowsArgs t = {};
+    t.q = a.q; t.cache = a.cache; t.part_out = a.part_out; t.part_lse = a.part_lse; t.items = a.items; t.members = a.members;
+    t.positions = a.positions; t.part_first = a.part_first; t.entry_slot = a.entry_slot; t.block_table = a.block_table;
+    t.hq = a.hq; t.hkv = a.hkv; t.page_size = a.page_size; t.num_pages = a.num_pages; t.max_pages = a.max_pages; t.slots = a.slots;
+    t.early = early ? 1 : 0; t.scale_log2 = a.scale_log2; t.slopes = a.slopes; t.fault = a.fault;
+    auto kernel = most_rows <= 8 ? (a.slopes != nullptr ? attention_rows_kernel<1, true> : attention_rows_kernel<1, false>)
+                                 : (a.slopes != nullptr ? attention_rows_kernel<2, true> : attention_rows_kernel<2, false>);
+    return launch_kernel(kernel, dim3(a.hkv, n_items), dim3(kRwWarps * 32), 0, stream, pdl, t);
+  }
 }
 
 static std::atomic<unsigned long long> g_shared_tc_configured[2][2];
@@ -1010,27 +997,24 @@ int rl_attention_shared(const void* q, const void* cache, void* out, float* part
         status = attn::launch_shared_tc(args, n_tile_items, tile_rows, pdl != 0, stream);
         if (status != 0) return status;
       }
-      if (n_row_items > 0) {
-        args.items = row_items;
-        status = attn::launch_listed_rows(args, n_row_items, most_rows, n_tile_items > 0, n_tile_items > 0 || pdl != 0, stream);
-        if (status != 0) return status;
-      }
     }
   }
-  if (tile_rows == 64) {
-    if (n_tile_items > 0) {
-      args.items = tile_items;
-      status = slopes != nullptr ? attn::launch_attention_as<4, 1, 2, false, true, true>(args, n_tile_items, pdl != 0, stream)
-                                 : attn::launch_attention_as<4, 1, 2, false, false, true>(args, n_tile_items, pdl != 0, stream);
-      if (status != 0) return status;
-    }
-    if (n_row_items > 0) {
-      args.items = row_items;
-      const bool dependent = n_tile_items > 0 || pdl != 0;
+  if (tile_rows == 64 && n_tile_items > 0) {
+    args.items = tile_items;
+    status = slopes != nullptr ? attn::launch_attention_as<4, 1, 2, false, true, true>(args, n_tile_items, pdl != 0, stream)
+                               : attn::launch_attention_as<4, 1, 2, false, false, true>(args, n_tile_items, pdl != 0, stream);
+    if (status != 0) return status;
+  }
+  if (n_row_items > 0) {
+    args.items = row_items;
+    const bool dependent = n_tile_items > 0 || pdl != 0;
+    if (attn::kRwTakes) {
+      status = attn::launch_rows(args, n_row_items, most_rows, n_tile_items > 0, dependent, stream);
+    } else {
       status = slopes != nullptr ? attn::launch_attention_as<1, 4, 3, false, true, true>(args, n_row_items, dependent, stream)
                                  : attn::launch_attention_as<1, 4, 3, false, false, true>(args, n_row_items, dependent, stream);
-      if (status != 0) return status;
     }
+    if (status != 0) return status;
   }
   const int rows = tokens * hq;
   return rl::launch_kernel(rl::attention_join_kernel<attn::bf16>, dim3((rows + rl::kJoinWarps - 1) / rl::kJoinWarps),

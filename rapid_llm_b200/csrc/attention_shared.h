@@ -29,10 +29,12 @@ constexpr int kListedFresh = 7;     // keys from here on are written by this ste
 // (item[0]: the entry whose block table is read)
 
 constexpr int kJoinWarps = 4;
+constexpr int kJoinAtOnce = 8;      // parts whose rows a lane has in flight
 
 // out[row] = sum_s w_s part[s] / (sum_s w_s + exp(sink)), w_s = 2^(lse_s - max): one warp a (token, head) row, parts
 // in index order, float32; the only rounding to the output's type is the last.  Four columns a lane, so that a part's row is
-// read as whole lines; kept in L2 by the kernels that wrote it.
+// read as whole lines.  A chain of latencies (the statistics, then the rows, both from L2) bounds it: the first eight rows are fetched
+// beside the statistics.  A part without keys counts nothing, whatever lies in its place.
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 attention_join_kernel(const float* part_out, const float* part_lse, const int* __restrict__ part_first, T* out,
@@ -43,44 +45,64 @@ attention_join_kernel(const float* part_out, const float* part_lse, const int* _
   const int token = mine ? row / hq : 0, head = mine ? row - token * hq : 0;
   const int first = part_first[token], parts = mine ? part_first[token + 1] - first : 0;
   const float sink2 = sink != nullptr ? sink[head] * 1.4426950408889634f : -INFINITY;
-  pdl_wait();
-  if (!mine) return;
   const float* lse = part_lse + static_cast<size_t>(first) * hq + head;
-  float top = sink2;
-  for (int s = lane; s < parts; s += 32) top = fmaxf(top, __ldcg(lse + static_cast<size_t>(s) * hq));
-  top = warp_max(top);
-  const float safe = top == -INFINITY ? 0.0f : top;
-  float total = lane == 0 && sink != nullptr ? exp2f(sink2 - safe) : 0.0f;
-  for (int s = lane; s < parts; s += 32) total += exp2f(__ldcg(lse + static_cast<size_t>(s) * hq) - safe);
-  total = warp_sum(total);
-  const float inv = (total > 0.0f ? 1.0f / total : 0.0f) * head_gate(gate, gate_stride, token, head);
   const float* src = part_out + (static_cast<size_t>(first) * hq + head) * d;
   T* dst = out + static_cast<size_t>(token) * out_stride + static_cast<size_t>(head) * d;
   const size_t step = static_cast<size_t>(hq) * d;
-  for (int c = lane * 4; c < d; c += 128) {
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = 0; s0 < parts; s0 += 4) {
-      float4 v[4];
-      float w[4];
+  pdl_wait();
+  if (!mine) return;
+  for (int c = lane * 4, turn = 0; turn * 128 < d; c += 128, ++turn) {
+    const bool in = c < d;
+    float4 v[kJoinAtOnce];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float l = s0 + i < parts ? __ldcg(lse + static_cast<size_t>(s0 + i) * hq) : -INFINITY;
-        w[i] = exp2f(l - safe);
-        // a part without keys counts nothing, whatever lies in its place
-        v[i] = l == -INFINITY ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : __ldcg(reinterpret_cast<const float4*>(src + (s0 + i) * step + c));
+    for (int i = 0; i < kJoinAtOnce; ++i)
+      v[i] = in && i < parts ? __ldcg(reinterpret_cast<const float4*>(src + i * step + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // a lane keeps the statistics of parts lane, lane + 32, ...: the maximum and the sum over all of them
+    const float l0 = lane < parts ? __ldcg(lse + static_cast<size_t>(lane) * hq) : -INFINITY;
+    float top = fmaxf(sink2, l0);
+    for (int s = lane + 32; s < parts; s += 32) top = fmaxf(top, __ldcg(lse + static_cast<size_t>(s) * hq));
+    top = warp_max(top);
+    const float safe = top == -INFINITY ? 0.0f : top;
+    const float w0 = exp2f(l0 - safe);
+    float total = w0;
+    for (int s = lane + 32; s < parts; s += 32) total += exp2f(__ldcg(lse + static_cast<size_t>(s) * hq) - safe);
+    total = warp_sum(total) + (sink != nullptr ? exp2f(sink2 - safe) : 0.0f);
+    const float inv = (total == 0.0f ? 0.0f : 1.0f / total) * head_gate(gate, gate_stride, token, head);      // a NaN stays one
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < parts; s0 += kJoinAtOnce) {
+      if (s0 > 0) {
+#pragma unroll
+        for (int i = 0; i < kJoinAtOnce; ++i)
+          v[i] = in && s0 + i < parts ? __ldcg(reinterpret_cast<const float4*>(src + (s0 + i) * step + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sum.x = fmaf(w[i], v[i].x, sum.x);
-        sum.y = fmaf(w[i], v[i].y, sum.y);
-        sum.z = fmaf(w[i], v[i].z, sum.z);
-        sum.w = fmaf(w[i], v[i].w, sum.w);
+      for (int i = 0; i < kJoinAtOnce; ++i) {
+        const int s = s0 + i;
+        const float w = s < 32 ? __shfl_sync(0xffffffffu, w0, s & 31) : s < parts ? exp2f(__ldcg(lse + static_cast<size_t>(s) * hq) - safe) : 0.0f;
+        if (w != 0.0f) {
+          sum.x = fmaf(w, v[i].x, sum.x);
+          sum.y = fmaf(w, v[i].y, sum.y);
+          sum.z = fmaf(w, v[i].z, sum.z);
+          sum.w = fmaf(w, v[i].w, sum.w);
+        }
       }
     }
-    dst[c] = from_float<T>(sum.x * inv);
-    dst[c + 1] = from_float<T>(sum.y * inv);
-    dst[c + 2] = from_float<T>(sum.z * inv);
-    dst[c + 3] = from_float<T>(sum.w * inv);
+    if (in) {
+      if constexpr (sizeof(T) == 2) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * inv, sum.y * inv), hi = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
+        uint2 both;
+        both.x = *reinterpret_cast<const uint32_t*>(&lo);
+        both.y = *reinterpret_cast<const uint32_t*>(&hi);
+        if ((reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+          *reinterpret_cast<uint2*>(dst + c) = both;
+          continue;
+        }
+      }
+      dst[c] = from_float<T>(sum.x * inv);
+      dst[c + 1] = from_float<T>(sum.y * inv);
+      dst[c + 2] = from_float<T>(sum.z * inv);
+      dst[c + 3] = from_float<T>(sum.w * inv);
+    }
   }
 }
 

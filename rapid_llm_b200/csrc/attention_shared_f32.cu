@@ -138,6 +138,7 @@ attention_shared_f32_kernel(const SharedF32Args args) {
       if (r0 < rows) {
         const float* qr = q_tile + r0 * stride;
         const float* kr = k_tile + k0 * stride;
+#pragma unroll 4
         for (int c = 0; c < d; c += 4) {
           const float4 k_a = *reinterpret_cast<const float4*>(kr + c), k_b = *reinterpret_cast<const float4*>(kr + 8 * stride + c);
 #pragma unroll
@@ -241,7 +242,7 @@ attention_shared_f32_kernel(const SharedF32Args args) {
       const size_t at = static_cast<size_t>(args.part_first[row_token[r]] + item[kListedPart]) * args.hq + head;
       *reinterpret_cast<float4*>(args.part_out + at * d + c) =
           make_float4(acc[u][i][0] * inv, acc[u][i][1] * inv, acc[u][i][2] * inv, acc[u][i][3] * inv);
-      if (c == 0) args.part_lse[at] = total > 0.0f ? row_max[r] + log2f(total) : -INFINITY;
+      if (c == 0) args.part_lse[at] = total == 0.0f ? -INFINITY : row_max[r] + log2f(total);
     }
   }
 }
@@ -278,7 +279,7 @@ int rl_attention_shared_f32(const float* q, const float* cache, float* out, floa
   }
   const int rows = tokens * hq;
   return rl::launch_kernel(rl::attention_join_kernel<float>, dim3((rows + rl::kJoinWarps - 1) / rl::kJoinWarps),
-                           dim3(rl::kJoinWarps * 32), 0, stream, pdl != 0, part_out, part_lse, part_first, out, rows, hq, d,
+                           dim3(rl::kJoinWarps * 32), 0, stream, pdl != 0 || n_items > 0, part_out, part_lse, part_first, out, rows, hq, d,
                            out_stride, sink, gate, gate_stride);
 }
 

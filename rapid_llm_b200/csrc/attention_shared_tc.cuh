@@ -16,7 +16,6 @@
 // for the kernel before.
 #pragma once
 
-#include "attention_decode_tc.cuh"
 #include "attention_prefill_tc.cuh"
 
 namespace rl {
@@ -37,6 +36,16 @@ constexpr int sh_stages(bool two_tiles) { return two_tiles ? 2 : 3; }
 constexpr int sh_smem_bytes(bool two_tiles) { return ((two_tiles ? 2 : 1) + 2 * sh_stages(two_tiles)) * kShTileBytes + 1024; }
 static_assert(2 * kShTileRows * kShOutStride * 4 <= sh_smem_bytes(true) - 1024 && kShTileRows * (kShOutStride + 2) * 4 <= sh_smem_bytes(false) - 1024,
               "the rows' results fit where the tiles were");
+
+// Rows `first` .. 127 of a tile of 128 keys (two halves of 128-byte rows) become zeros, by one warp, for the tensor cores to see.
+__device__ __forceinline__ void sh_clear_rows(uint32_t tile, int first, int lane) {
+  for (int i = first * 16 + lane; i < kShKeys * 16; i += 32) {
+    const uint32_t at = tile + ((i >> 3) & 1) * kShHalfBytes + (i >> 4) * 128 + (i & 7) * 16;
+    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(at), "r"(0) : "memory");
+  }
+  fence_async_smem();
+  __syncwarp();
+}
 
 struct SharedTcArgs {
   const bf16* q;
@@ -240,7 +249,7 @@ attention_shared_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
         ok = wait(&p_ready[st], j) && wait(&full_v[stage], b / kStages);
         if (!ok) break;
         // what came along beyond the keys' end is cleared before its first use: zero times a NaN is no zero
-        if (b == n_blocks - 1 && kb_end > k_end && (!kTwoTiles || st == 0)) clear_rows(v_tile(stage), k_end - (kb_end - kShKeys), lane);
+        if (b == n_blocks - 1 && kb_end > k_end && (!kTwoTiles || st == 0)) sh_clear_rows(v_tile(stage), k_end - (kb_end - kShKeys), lane);
         tc_fence_after();
         const uint64_t values_desc = operand_desc_mn(v_tile(stage), kShHalfBytes);
         if (issues) {
@@ -461,7 +470,7 @@ attention_shared_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
         }
         if (valid)
           args.part_lse[static_cast<size_t>(args.part_first[token] + part) * args.hq + head] =
-              row_sum > 0.0f ? top + log2f(row_sum) : -INFINITY;
+              row_sum == 0.0f ? -INFINITY : top + log2f(row_sum);
       }
       named_barrier(1, 256);
       // whole rows of 512 bytes, a warp a row

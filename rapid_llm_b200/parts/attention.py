@@ -243,13 +243,44 @@ class SharedItems(StepPlanner):
     def __init__(self, group: int, num_kv_heads: int, head_dim: int, sms: int = DEFAULT_SMS, dtype: torch.dtype = torch.bfloat16) -> None:
         self.group, self.num_kv_heads, self.head_dim, self.sms = int(group), int(num_kv_heads), int(head_dim), int(sms)
         self.wide = dtype == torch.float32
-        self.ctas_per_sm = 2
         self.tag = kernels.dtype_tag(dtype)
         self.key = ("shared_items", self.group, self.num_kv_heads, self.head_dim, self.sms, self.tag)
 
     def part_rows(self, plan: dict) -> int:
         """Rows of the two scratch buffers."""
         return plan["parts"] * self.group * self.num_kv_heads
+
+    # What an item takes, in units of a microsecond: a start (page ids, queries, the first keys, the result) and so much a block of 128
+    # keys; how many items of a kind a multiprocessor runs at one time.  By the kind of tile: rows of a tile -> (start, block, together).
+    COSTS = {256: (6.0, 2.4, 1), 128: (6.0, 1.3, 1), 64: (4.0, 1.2, 2), 32: (5.0, 5.0, 2), 16: (3.0, 1.0, 3)}
+
+    def _blocks_per_item(self, tiles, rows, tile_rows: int) -> tuple[int, int]:
+        """Blocks of keys that a tile item and a row item take, for lists of (blocks, items side by side): so few that all
+        multiprocessors have work, and so many that the items, each with a start of its own and a part of its rows' results
+        to join, run at one time.  Of the steps tried the one whose longest item, or whose sum over the multiprocessors, is
+        done first."""
+        tile_start, tile_block, tile_together = self.COSTS[tile_rows]
+        row_start, row_block, row_together = self.COSTS[kernels.DECODE_TILE_ROWS]
+        longest = max([blocks for blocks, _ in [*tiles, *rows]] or [1])
+        steps = sorted({min(longest, step) for step in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 28, 32, 40, 48, 64, 96, 128, 192, 256, 512, 1024)})
+        best, chosen = None, (longest, longest)
+        row_steps = steps if rows else steps[:1]
+        for row_step in row_steps:
+            row_items = sum(-(-blocks // row_step) * side for blocks, side in rows)
+            row_time = sum(row_start * -(-blocks // row_step) * side + row_block * blocks * side for blocks, side in rows) / row_together
+            row_end = max([row_start + row_block * min(row_step, blocks) for blocks, _ in rows] or [0.0])
+            for step in steps if tiles else steps[:1]:
+                tile_items = sum(-(-blocks // step) * side for blocks, side in tiles)
+                tile_time = sum(tile_start * -(-blocks // step) * side + tile_block * blocks * side for blocks, side in tiles) / tile_together
+                tile_end = max([tile_start + tile_block * min(step, blocks) for blocks, _ in tiles] or [0.0])
+                waves = -(-tile_items // (self.sms * tile_together)) * tile_end
+                most_parts = max([-(-blocks // step) for blocks, _ in tiles] or [0]) + max([-(-blocks // row_step) for blocks, _ in rows] or [0])
+                end = max((row_time + tile_time) / self.sms, row_end, waves) + 0.15 * most_parts
+                if row_items > 60000 or tile_items > 60000:
+                    continue
+                if best is None or end < best - 1e-9:
+                    best, chosen = end, (step, row_step)
+        return chosen
 
     def plan(self, shape: StepShape) -> dict:
         lengths, starts = np.asarray(shape.lengths, dtype=np.int64), np.asarray(shape.starts, dtype=np.int64)
@@ -290,20 +321,21 @@ class SharedItems(StepPlanner):
             tile_rows = kernels.SHARED_TC_ROWS[max(packed_rows) > kernels.SHARED_TC_ROWS[0]]
 
         def height_of(rows: int) -> int:
-            if not self.wide and rows <= kernels.DECODE_TILE_ROWS:
-                return kernels.DECODE_TILE_ROWS
-            tiles = -(-rows // tile_rows)
-            return min(tile_rows, -(-(-(-rows // tiles)) // 32) * 32)       # even tiles of whole warps
+            return kernels.DECODE_TILE_ROWS if not self.wide and rows <= kernels.DECODE_TILE_ROWS else tile_rows
 
-        units = sum(-(-(end - first) // block) * -(-rows // height_of(rows))
-                    for (_, first, end, _, _, _, _), rows in zip(work, packed_rows)) * self.num_kv_heads
-        per_item = max(1, -(-units // (self.ctas_per_sm * self.sms)))       # blocks of keys an item takes
+        is_row = [not self.wide and rows <= kernels.DECODE_TILE_ROWS for rows in packed_rows]
+        tile_step, row_step = self._blocks_per_item(
+            [(-(-(end - first) // block), -(-rows // height_of(rows)) * self.num_kv_heads) for (_, first, end, _, _, _, _), rows, low
+             in zip(work, packed_rows, is_row) if not low],
+            [(-(-(end - first) // block), -(-rows // kernels.DECODE_TILE_ROWS) * self.num_kv_heads) for (_, first, end, _, _, _, _), rows, low
+             in zip(work, packed_rows, is_row) if low], tile_rows)
         parts = np.zeros(tokens, dtype=np.int64)                # of each token so far: a group's items come before its entries'
         tiles, rows, most = [], [], 0
         for entry, first, end, member, n, fresh, its in work:
             packed = n * self.group
             height = height_of(packed)
-            bucket = rows if not self.wide and packed <= kernels.DECODE_TILE_ROWS else tiles
+            low_item = not self.wide and packed <= kernels.DECODE_TILE_ROWS
+            bucket, per_item = (rows, row_step) if low_item else (tiles, tile_step)
             if bucket is rows:
                 most = max(most, min(height, packed))
             ranges = max(1, -(-(end - first) // (per_item * block)))

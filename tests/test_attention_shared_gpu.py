@@ -281,3 +281,21 @@ def test_long_keys_of_their_own_walked_by_one_item(own):
     want = step.want()
     for _ in range(4):
         check(step.run(), want, torch.bfloat16, 128)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 128)])
+def test_a_nan_that_is_seen_stays_one(dtype, dim):
+    """In a request's own key: its rows; in a shared one: every row of the group; nowhere else."""
+    for members in (3, 40):
+        step = Step([160, 48], [(0, 1 + 7 * i % 40, 1) for i in range(members)] + [(1, 3, 1), (-1, 130, 1)], heads=4, kv_heads=2, dim=dim,
+                    page=16, dtype=dtype, seed=3)
+        clean = step.run()
+        own_page = int(step.table[step.slots[1], step.positions[1] // 16])
+        step.cache[own_page, 0, 0, step.positions[1] % 16] = float("nan")
+        got = step.run().view(-1, 4, dim)
+        assert bool(got[1, :2].isnan().all()) and not bool(got[1, 2:].isnan().any())
+        got[1] = clean.view(-1, 4, dim)[1]
+        assert torch.equal(got.view(clean.shape), clean)
+        step.cache[int(step.table[step.slots[0], 4]), 0, 1, 5] = float("nan")
+        got = step.run().view(-1, 4, dim)
+        assert bool(got[:members, 2:].isnan().all()) and torch.equal(got[members:], clean.view(-1, 4, dim)[members:])
