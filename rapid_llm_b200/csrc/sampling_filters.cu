@@ -94,19 +94,19 @@ __device__ __forceinline__ void philox_words(uint32_t (&c)[4], uint32_t k0, uint
   }
 }
 
-// w = rint(2^43 exp((x - top) / T)): 2^(t / 64) with t = (x - top) * 64 log2(e) / T as 2^(j / 64) from a table, 2^e in
-// the exponent, and the rest, at most 1 / 128 of an octave, as its series to the fifth power (remainder 6e-17).
-__device__ __forceinline__ u64 weight_of(float x, float top, float floor_value, double per, const double* table) {
+// w = rint(2^43 exp((x - top) / T)): with t = (x - top) 64 log2(e) / T, 2^(t / 64) is 2^(j / 64) from a table, 2^e in the
+// exponent, and the rest, at most 1 / 128 of an octave, as its series to the fourth power (remainder 4e-14, a third of the unit).
+__device__ __forceinline__ u64 weight_of(float x, double top, float floor_value, double per, const double* table) {
   if (!(x >= floor_value)) return 0ull;
-  const double t = (static_cast<double>(x) - static_cast<double>(top)) * per;
+  const double t = (static_cast<double>(x) - top) * per;
   const double shifted = t + 6755399441055744.0;                       // 1.5 * 2^52: the nearest whole number in the low bits
   const int m = __double2loint(shifted);
   if (m < -64 * 60) return 0ull;
-  const double f = (t - (shifted - 6755399441055744.0)) * 0.010830424696249145;      // ln 2 / 64
-  double p = fma(f, 1.0 / 120.0, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
+  const double f = t - (shifted - 6755399441055744.0);
+  constexpr double a = 0.010830424696249145;                           // ln 2 / 64
+  double p = fma(f, a * a * a * a / 24.0, a * a * a / 6.0);
+  p = fma(p, f, a * a / 2.0);
+  p = fma(p, f, a);
   p = fma(p, f, 1.0);
   p *= table[m & 63];
   const double scaled = __hiloint2double(__double2hiint(p) + (((m >> 6) + 43) << 20), __double2loint(p));
@@ -120,11 +120,11 @@ struct Shared {
   unsigned counts[kBins];
   double table[64];
   u64 share[2][4];                // partial results for the peers
-  u64 warp_sums[kWarps];
-  unsigned warp_words[kWarps];
+  u64 theirs[2][kMaxRanks][4];    // the peers' results
+  u64 warp_sums[4][kWarps];
   float list_x[kList];            // this CTA's tokens of the interval
   int list_i[kList];
-  unsigned list_n;
+  unsigned list_n, list_of[kMaxRanks];
   float all_x[kList];             // the cluster's
   int all_i[kList];
   u64 all_w[kList];
@@ -146,70 +146,85 @@ struct Row {
   int turn = 0;                 // of the exchange buffers
   int level = 0;                // of the histogram buffers
   float top, floor_value, code_scale;
-  double per;
+  double per, wide_top;
 
   __device__ Row(Shared& shared, float* v) : s(shared), values(v) {}
 
-  // ---- reductions: over the CTA, then over the cluster; every thread gets the result -------------------------
-  __device__ u64 block_sum(u64 v) {
+  // ---- reductions: over the CTA, then over the cluster; every thread gets the results -------------------------
+  struct Sum { __device__ static u64 of(u64 a, u64 b) { return a + b; } };
+  struct Most { __device__ static u64 of(u64 a, u64 b) { return a > b ? a : b; } };
+  template <typename Op, int kCount>
+  __device__ void block_all(u64 (&v)[kCount]) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s.warp_sums[threadIdx.x >> 5] = v;
-    __syncthreads();
-    u64 total = 0;
+    for (int k = 0; k < kCount; ++k)
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) total += s.warp_sums[w];
-    return total;
+      for (int o = 16; o > 0; o >>= 1) v[k] = Op::of(v[k], __shfl_xor_sync(0xffffffffu, v[k], o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int k = 0; k < kCount; ++k) s.warp_sums[k][threadIdx.x >> 5] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+      v[k] = s.warp_sums[k][threadIdx.x & (kWarps - 1)];
+#pragma unroll
+      for (int o = kWarps / 2; o > 0; o >>= 1) v[k] = Op::of(v[k], __shfl_xor_sync(0xffffffffu, v[k], o));
+    }
   }
-  __device__ unsigned block_max(unsigned v) {
-    v = __reduce_max_sync(0xffffffffu, v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s.warp_words[threadIdx.x >> 5] = v;
-    __syncthreads();
-    unsigned best = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) best = max(best, s.warp_words[w]);
-    return best;
-  }
-  // The peers' words of this exchange.  A buffer is written again two exchanges later, when every rank has passed the
-  // barrier between and so read this one.
-  template <typename Fn>
-  __device__ void exchange(u64 a, u64 b, Fn&& each) {
+  // The CTAs' words of this exchange, fetched by a few lanes for all.  A buffer is written again two exchanges later, when
+  // every rank has passed the barrier between and so read this one.
+  template <int kCount>
+  __device__ const u64 (*exchange(const u64 (&v)[kCount]))[4] {
     const int slot = turn++ & 1;
     if (threadIdx.x == 0) {
-      s.share[slot][0] = a;
-      s.share[slot][1] = b;
+#pragma unroll
+      for (int k = 0; k < kCount; ++k) s.share[slot][k] = v[k];
     }
-    if (ranks == 1) {
+    if (ranks > 1) {
+      cluster_barrier();
+    } else {
       __syncthreads();
-      each(0u, s.share[slot][0], s.share[slot][1]);
-      return;
     }
-    cluster_barrier();
-    for (unsigned r = 0; r < ranks; ++r) each(r, peer_u64(&s.share[slot][0], r), peer_u64(&s.share[slot][1], r));
+    if (threadIdx.x < ranks * kCount) {
+      const unsigned r = threadIdx.x / kCount, k = threadIdx.x % kCount;
+      s.theirs[slot][r][k] = ranks > 1 ? peer_u64(&s.share[slot][k], r) : s.share[slot][k];
+    }
+    __syncthreads();
+    return s.theirs[slot];
+  }
+  template <typename Op, int kCount>
+  __device__ void cluster_all(u64 (&v)[kCount]) {
+    block_all<Op>(v);
+    const u64(*all)[4] = exchange(v);
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) v[k] = all[0][k];
+    for (unsigned r = 1; r < ranks; ++r)
+#pragma unroll
+      for (int k = 0; k < kCount; ++k) v[k] = Op::of(v[k], all[r][k]);
+  }
+  __device__ u64 block_sum(u64 v) {
+    u64 one[1] = {v};
+    block_all<Sum>(one);
+    return one[0];
   }
   __device__ u64 cluster_sum(u64 v) {
-    u64 total = 0;
-    exchange(block_sum(v), 0, [&](unsigned, u64 a, u64) { total += a; });
-    return total;
-  }
-  __device__ unsigned cluster_max(unsigned v) {
-    unsigned best = 0;
-    exchange(block_max(v), 0, [&](unsigned, u64 a, u64) { best = max(best, static_cast<unsigned>(a)); });
-    return best;
+    u64 one[1] = {v};
+    cluster_all<Sum>(one);
+    return one[0];
   }
 
   template <typename Fn>
   __device__ __forceinline__ void sweep(Fn&& fn) {
     const int first = min(count, static_cast<int>(threadIdx.x) * chunk), last = min(count, first + chunk);
+#pragma unroll 4
     for (int i = first; i < last; ++i) fn(i, values[i]);
   }
   // 23-bit code of the distance to the maximum, or more than that for what lies outside
   __device__ __forceinline__ unsigned code(float x) const {
     return __float_as_uint(fmaf(top - x, code_scale, 8388608.0f)) - 0x4B000000u;
   }
-  __device__ __forceinline__ u64 weight(float x) const { return weight_of(x, top, floor_value, per, s.table); }
+  __device__ __forceinline__ u64 weight(float x) const { return weight_of(x, wide_top, floor_value, per, s.table); }
 
   struct Interval {
     unsigned low, high;         // codes, both included
@@ -345,8 +360,8 @@ struct Row {
     __syncthreads();
   }
 
-  // Tokens of the cluster with codes low .. high (at most kList of them) into all_x, all_i, all_w of every CTA, in
-  // index order of the ranks; returns how many.
+  // Tokens of the cluster with codes low .. high (at most kList of them) into all_x, all_i, all_w of every CTA; returns how
+  // many.  A rank's list may be written again only behind a barrier of the cluster (no call gathers twice without one).
   template <typename In>
   __device__ unsigned gather(unsigned low, unsigned high, In&& in) {
     if (threadIdx.x == 0) s.list_n = 0;
@@ -362,20 +377,21 @@ struct Row {
     });
     __syncthreads();
     if (ranks > 1) cluster_barrier();
-    unsigned first = 0;
-    for (unsigned r = 0; r < ranks; ++r) {
-      const unsigned n = min(ranks == 1 ? s.list_n : peer_u32(&s.list_n, r), static_cast<unsigned>(kList));
-      for (unsigned j = threadIdx.x; j < n && first + j < kList; j += kThreads) {
-        const float x = ranks == 1 ? s.list_x[j] : __uint_as_float(peer_u32(&s.list_x[j], r));
-        s.all_x[first + j] = x;
-        s.all_i[first + j] = ranks == 1 ? s.list_i[j] : static_cast<int>(peer_u32(&s.list_i[j], r));
-        s.all_w[first + j] = weight(x);
-      }
-      first += n;
-    }
-    if (ranks > 1) cluster_barrier();               // the lists may be written again
+    if (threadIdx.x < ranks) s.list_of[threadIdx.x] = ranks == 1 ? s.list_n : peer_u32(&s.list_n, threadIdx.x);
     __syncthreads();
-    return min(first, static_cast<unsigned>(kList));
+    unsigned all = 0;
+    for (unsigned r = 0; r < ranks; ++r) all += min(s.list_of[r], static_cast<unsigned>(kList));
+    all = min(all, static_cast<unsigned>(kList));
+    if (threadIdx.x < all) {
+      unsigned r = 0, j = threadIdx.x;
+      while (j >= s.list_of[r]) j -= s.list_of[r++];
+      const float x = ranks == 1 ? s.list_x[j] : __uint_as_float(peer_u32(&s.list_x[j], r));
+      s.all_x[threadIdx.x] = x;
+      s.all_i[threadIdx.x] = ranks == 1 ? s.list_i[j] : static_cast<int>(peer_u32(&s.list_i[j], r));
+      s.all_w[threadIdx.x] = weight(x);
+    }
+    __syncthreads();
+    return all;
   }
 
   // The largest and smallest value among the tokens of an interval.
@@ -388,10 +404,20 @@ struct Row {
       high = max(high, ordered(x));
       low = max(low, ~ordered(x));
     });
-    most = unordered(cluster_max(high));
-    least = unordered(~cluster_max(low));
+    u64 ends[2] = {high, low};
+    cluster_all<Most>(ends);
+    most = unordered(static_cast<unsigned>(ends[0]));
+    least = unordered(~static_cast<unsigned>(ends[1]));
   }
 };
+
+constexpr int kRoomySlice = 24 * 1024;        // floats of a slice of which two fit a multiprocessor
+
+static int sm_count() {
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 148;
+  return sms;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -417,16 +443,44 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   const T* x = static_cast<const T*>(args.logits) + static_cast<size_t>(row_index) * args.row_stride + row.begin;
   const bool vector = (reinterpret_cast<uintptr_t>(x) & (sizeof(T) == 2 ? 15 : 31)) == 0;
   const int vector_count = vector ? (row.count & ~7) : 0;
-  auto clean = [](float v) { return v == v ? v : -INFINITY; };
-  for (int c = threadIdx.x * 8; c < vector_count; c += kThreads * 8) {
-    float v[8];
-    load8(x + c, v);
+  auto clean = [](float v) { return v == v ? v + 0.0f : -INFINITY; };      // (the sum makes a negative zero the zero it equals)
+  // the largest value with the first index it has (as a complement), and the smallest finite one, on the way
+  u64 ends[2] = {0ull, 0ull};
+  auto seen = [&](int i, float v) {
+    const unsigned k = ordered(v);
+    ends[0] = max(ends[0], static_cast<u64>(k) << 32 | ~static_cast<unsigned>(row.begin + i));
+    if (v > -INFINITY) ends[1] = max(ends[1], static_cast<u64>(~k));
+  };
+  const bool penalised = pen != 1.0f && args.seen_tokens != nullptr && seen_end > seen_begin;
+  constexpr int kFly = sizeof(T) == 2 ? 5 : 3;       // 8-element loads of a thread in flight, kept as they come
+  struct alignas(16) Raw { uint4 word[sizeof(T) == 2 ? 1 : 2]; };
+  for (int c0 = threadIdx.x * 8; c0 < vector_count; c0 += kFly * kThreads * 8) {
+    Raw raw[kFly];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) slice_values[c + j] = clean(v[j]);
+    for (int f = 0; f < kFly; ++f)
+      if (c0 + f * kThreads * 8 < vector_count) raw[f] = *reinterpret_cast<const Raw*>(x + c0 + f * kThreads * 8);
+#pragma unroll
+    for (int f = 0; f < kFly; ++f) {
+      const int c = c0 + f * kThreads * 8;
+      if (c >= vector_count) break;
+      float v[8];
+      const T* values = reinterpret_cast<const T*>(&raw[f]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = clean(to_float(values[j]));
+        if (!penalised) seen(c + j, v[j]);
+      }
+      *reinterpret_cast<float4*>(slice_values + c) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(slice_values + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    }
   }
-  for (int i = vector_count + threadIdx.x; i < row.count; i += kThreads) slice_values[i] = clean(to_float(x[i]));
+  for (int i = vector_count + threadIdx.x; i < row.count; i += kThreads) {
+    const float v = clean(to_float(x[i]));
+    slice_values[i] = v;
+    if (!penalised) seen(i, v);
+  }
   __syncthreads();
-  if (pen != 1.0f && args.seen_tokens != nullptr && seen_end > seen_begin) {
+  if (penalised) {
     // every generated token once: the first of equal ids in the list applies the penalty
     for (int i = seen_begin + threadIdx.x; i < seen_end; i += kThreads) {
       const int id = args.seen_tokens[i] - row.begin;
@@ -439,34 +493,17 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       }
     }
     __syncthreads();
+    row.sweep(seen);
   }
-
-  // ---- the first maximum, the smallest finite value ------------------------------------------------------------
-  unsigned most = 0, least = 0;
-  int place = 0x7fffffff;
-  row.sweep([&](int i, float v) {
-    const unsigned k = ordered(v);
-    if (k > most) {
-      most = k;
-      place = row.begin + i;
-    }
-    if (v > -INFINITY) least = max(least, ~k);
-  });
-  const unsigned mine = most;
-  most = row.cluster_max(most);
-  const unsigned first_at = ~row.cluster_max(mine == most && row.count > 0 ? ~static_cast<unsigned>(place) : 0u);
-  float top = unordered(most);
-  if (!(top > -INFINITY)) {                          // nothing to choose from
-    if (row.rank == 0 && threadIdx.x == 0) args.out[row_index] = 0;
+  row.template cluster_all<typename Row<T>::Most>(ends);
+  float top = unordered(static_cast<unsigned>(ends[0] >> 32));
+  if (ends[0] == 0ull || !(top > -INFINITY) || !(temp > 0.0f)) {
+    // nothing to choose from, or the first maximum; nobody leaves while its shared memory may be read
+    if (row.rank == 0 && threadIdx.x == 0) args.out[row_index] = top > -INFINITY ? static_cast<int>(~static_cast<unsigned>(ends[0])) : 0;
     if (ranks > 1) cluster_barrier();
     return;
   }
-  if (!(temp > 0.0f)) {
-    if (row.rank == 0 && threadIdx.x == 0) args.out[row_index] = static_cast<int>(first_at);
-    if (ranks > 1) cluster_barrier();                // nobody leaves while its shared memory may be read
-    return;
-  }
-  float bottom = unordered(~row.cluster_max(least));
+  float bottom = unordered(~static_cast<unsigned>(ends[1]));
   if (top == INFINITY) {                             // entries of +infinity share everything
     row.sweep([&](int i, float v) { slice_values[i] = v == INFINITY ? 0.0f : -INFINITY; });
     top = bottom = 0.0f;
@@ -475,6 +512,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   row.top = top;
   row.floor_value = fmaxf(top - kNegligible * temp, -3.4028235e38f);
   row.per = 92.33248261893585 / static_cast<double>(temp);       // 64 log2(e) / T
+  row.wide_top = static_cast<double>(top);
   {
     // codes: the distance times a power of two, so that the farthest that counts stays below 2^23
     const float farthest = fminf(top - bottom, kNegligible * temp * 1.01f);
@@ -527,36 +565,40 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
     } else if (at.above_n + at.inside_n <= kList) {
       // the whole of top-k and a little more fits the list: everything else happens there
       const unsigned n = row.gather(0u, at.high, everything);
-      const bool have = threadIdx.x < n;
-      const float my_x = have ? s.all_x[threadIdx.x] : 0.0f;
-      const int my_i = have ? s.all_i[threadIdx.x] : 0;
-      const u64 my_w = have ? s.all_w[threadIdx.x] : 0ull;
-      unsigned rank = 0;
-      if (have)
-        for (unsigned j = 0; j < n; ++j) rank += s.all_x[j] > my_x || (s.all_x[j] == my_x && s.all_i[j] < my_i);
-      bool keep = have && rank < static_cast<unsigned>(want_k);
-      if (have) s.all_keep[threadIdx.x] = keep;
-      const u64 z = row.block_sum(keep ? my_w : 0ull);
-      __syncthreads();
-      if (keep && by_mass) {
+      // (the same in every CTA).  Each token is compared with all others by `side` neighbouring lanes.
+      const unsigned padded = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256, side = kThreads / padded;
+      const unsigned mine = threadIdx.x / side, sub = threadIdx.x % side;
+      const bool have = mine < n, lead = sub == 0;
+      const float my_x = have ? s.all_x[mine] : 0.0f;
+      const int my_i = have ? s.all_i[mine] : 0;
+      const u64 my_w = have ? s.all_w[mine] : 0ull;
+      auto over_side = [&](u64 v) {
+        for (unsigned o = 1; o < side; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+      };
+      u64 rank = 0;
+      for (unsigned j = sub; j < n; j += side) rank += s.all_x[j] > my_x || (s.all_x[j] == my_x && s.all_i[j] < my_i);
+      rank = over_side(rank);                        // (every lane takes part)
+      bool keep = have && rank < static_cast<u64>(want_k);
+      if (by_mass) {
+        if (lead && have) s.all_keep[mine] = keep;
+        const u64 z = row.block_sum(lead && keep ? my_w : 0ull);       // (its barriers publish the marks)
         u64 above = 0;
-        for (unsigned j = 0; j < n; ++j) above += s.all_keep[j] && s.all_x[j] > my_x ? s.all_w[j] : 0ull;
-        keep = static_cast<double>(above) <= static_cast<double>(p) * static_cast<double>(z) || my_x == top;
+        for (unsigned j = sub; j < n; j += side) above += s.all_keep[j] && s.all_x[j] > my_x ? s.all_w[j] : 0ull;
+        above = over_side(above);
+        keep = keep && (static_cast<double>(above) <= static_cast<double>(p) * static_cast<double>(z) || my_x == top);
+        __syncthreads();
       }
       keep = keep && (static_cast<double>(my_w) >= least_weight) && (my_w > 0 || (first_of_all && counts_at_all(my_x)));
-      __syncthreads();
-      if (have) s.all_keep[threadIdx.x] = keep;
-      const u64 mass = row.block_sum(keep ? my_w : 0ull);
-      __syncthreads();
-      if (keep && first_of_all) {
-        bool first = true;
-        for (unsigned j = 0; j < n; ++j) first = first && !(s.all_keep[j] && s.all_i[j] < my_i);
-        if (first && row.rank == 0) args.out[row_index] = my_i;
-      } else if (keep) {
-        const u64 target = target_of(mass);
-        u64 before = 0;
-        for (unsigned j = 0; j < n; ++j) before += s.all_keep[j] && s.all_i[j] < my_i ? s.all_w[j] : 0ull;
-        if (row.rank == 0 && before <= target && target < before + my_w) args.out[row_index] = my_i;
+      if (lead && have) s.all_keep[mine] = keep;
+      const u64 mass = row.block_sum(lead && keep ? my_w : 0ull);
+      u64 before = 0;
+      for (unsigned j = sub; j < n; j += side)
+        before += s.all_keep[j] && s.all_i[j] < my_i ? (first_of_all ? 1ull : s.all_w[j]) : 0ull;
+      before = over_side(before);
+      if (keep && lead && row.rank == 0) {
+        const u64 target = first_of_all ? 0ull : target_of(mass);
+        if (before <= target && target < before + (first_of_all ? 1ull : my_w)) args.out[row_index] = my_i;
       }
       if (ranks > 1) cluster_barrier();
       return;
@@ -605,6 +647,8 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
 
   // ---- top-p: the smallest value that stays ----------------------------------------------------------------------------
   float cut_p = -INFINITY;
+  u64 weighed = 0;                                   // of this thread's chunk: the mass of codes below `weighed_to`, all of which stays
+  unsigned weighed_to = 0;
   if (by_mass) {
     typename Row<T>::Interval at = {0u, kLast, 0u, 0u, 0.0};
     double whole = -1.0;
@@ -613,9 +657,22 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       if (at.inside_n <= kList || at.low == at.high) break;
     }
     float high, low;
-    row.range_of(at, in_k, high, low);
+    unsigned listed = 0;
+    if (at.inside_n > kList) {
+      row.range_of(at, in_k, high, low);
+    } else {
+      listed = row.gather(at.low, at.high, in_k);
+      u64 ends_of[2] = {0ull, 0ull};
+      if (threadIdx.x < listed) {
+        ends_of[0] = ordered(s.all_x[threadIdx.x]);
+        ends_of[1] = ~ordered(s.all_x[threadIdx.x]);
+      }
+      row.template block_all<typename Row<T>::Most>(ends_of);
+      high = unordered(static_cast<unsigned>(ends_of[0]));
+      low = unordered(~static_cast<unsigned>(ends_of[1]));
+    }
     if (high == low) {
-      cut_p = high;
+      cut_p = high;                                  // one value, as often as it may be there
     } else {
       // exact sums from here on: the whole mass, what lies before the interval and in it
       u64 z = 0, above = 0, inside = 0, behind = 0;
@@ -628,17 +685,25 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
         else if (q <= at.high) inside += w;
         else if (q <= kLast) behind += 1;
       });
-      z = row.cluster_sum(z);
-      above = row.cluster_sum(above);
-      inside = row.cluster_sum(inside);
-      behind = row.cluster_sum(behind);
+      u64 sums[4] = {z, above, inside, behind};
+      row.template cluster_all<typename Row<T>::Sum>(sums);
+      weighed = above;
+      weighed_to = at.low;
+      z = sums[0];
+      above = sums[1];
+      inside = sums[2];
+      behind = sums[3];
       const double budget = fmax(static_cast<double>(p), 0.0) * static_cast<double>(z);
       if (static_cast<double>(above) > budget) {       // (not met: the approximate masses are nearer than their slack)
         at = {0u, at.low - 1u, 0u, at.above_n, 0.0};
         above = 0;
+        weighed = 0;
+        weighed_to = 0;
+        listed = 0;
       } else if (static_cast<double>(above + inside) <= budget && behind > 0) {
         at = {at.high + 1u, kLast, at.above_n + at.inside_n, static_cast<unsigned>(behind), 0.0};
         above += inside;
+        listed = 0;
       }
       // halve the interval until the list holds it: its far half if that one's first token stays
       while (at.inside_n > kList && at.low < at.high) {
@@ -650,8 +715,10 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
           near_mass += row.weight(v);
           near_n += 1;
         });
-        near_mass = row.cluster_sum(near_mass);
-        near_n = row.cluster_sum(near_n);
+        u64 near_sums[2] = {near_mass, near_n};
+        row.template cluster_all<typename Row<T>::Sum>(near_sums);
+        near_mass = near_sums[0];
+        near_n = near_sums[1];
         if (static_cast<double>(above + near_mass) <= budget && near_n < at.inside_n) {
           above += near_mass;
           at.low = mid + 1u;
@@ -662,7 +729,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
         }
       }
       if (at.inside_n <= kList) {
-        const unsigned n = row.gather(at.low, at.high, in_k);
+        const unsigned n = listed > 0 ? listed : row.gather(at.low, at.high, in_k);
         unsigned best = 0;                             // the smallest that stays, as the largest of the complements
         if (threadIdx.x < n) {
           const float my_x = s.all_x[threadIdx.x];
@@ -670,7 +737,9 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
           for (unsigned j = 0; j < n; ++j) mass += s.all_x[j] > my_x ? s.all_w[j] : 0ull;
           if (static_cast<double>(mass) <= budget) best = ~ordered(my_x);
         }
-        cut_p = unordered(~row.block_max(best));
+        u64 one[1] = {best};
+        row.template block_all<typename Row<T>::Most>(one);
+        cut_p = unordered(~static_cast<unsigned>(one[0]));
         __syncthreads();
       } else {
         // more than that within one code: by their values, the smallest v with mass(x > v) <= budget
@@ -696,19 +765,29 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       if (best == 0 && v > -INFINITY && v >= cut_p && in_k(i, v) && counts_at_all(v) && static_cast<double>(row.weight(v)) >= least_weight)
         best = ~static_cast<unsigned>(row.begin + i);
     });
-    best = row.cluster_max(best);
-    if (row.rank == 0 && threadIdx.x == 0) args.out[row_index] = static_cast<int>(~best);
+    u64 one[1] = {best};
+    row.template cluster_all<typename Row<T>::Most>(one);
+    if (row.rank == 0 && threadIdx.x == 0) args.out[row_index] = static_cast<int>(~static_cast<unsigned>(one[0]));
     if (ranks > 1) cluster_barrier();
     return;
   }
-  const float lower = fmaxf(fmaxf(cut_p, row.floor_value), -3.4028235e38f);
+  // (min-p's own cut, drawn a little wide, spares most weights their exponential)
+  const float cut_min = least_p > 0.0f ? top + temp * (logf(least_p) * 1.001f - 0.001f) : -3.4028235e38f;
+  const float lower = fmaxf(fmaxf(cut_p, row.floor_value), fmaxf(cut_min, -3.4028235e38f));
   auto kept_weight = [&](int i, float v) -> u64 {
     if (v < lower || !in_k(i, v)) return 0ull;
     const u64 w = row.weight(v);
     return static_cast<double>(w) >= least_weight ? w : 0ull;
   };
   u64 local = 0;
-  row.sweep([&](int i, float v) { local += kept_weight(i, v); });
+  if (weighed_to > 0 && least_p <= 0.0f) {
+    local = weighed;
+    row.sweep([&](int i, float v) {
+      if (v >= lower && row.code(v) >= weighed_to) local += kept_weight(i, v);
+    });
+  } else {
+    row.sweep([&](int i, float v) { local += kept_weight(i, v); });
+  }
   // running sums in index order: over the thread's chunk, the warp, the CTA, the ranks
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 upto = local;
@@ -718,19 +797,21 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
     if (lane >= o) upto += up;
   }
   __syncthreads();
-  if (lane == 31) s.warp_sums[warp] = upto;
+  if (lane == 31) s.warp_sums[0][warp] = upto;
   __syncthreads();
   u64 cta = 0, base = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) base += s.warp_sums[w];
-    cta += s.warp_sums[w];
+    if (w < warp) base += s.warp_sums[0][w];
+    cta += s.warp_sums[0][w];
   }
   u64 mass = 0, front = 0;
-  row.exchange(cta, 0, [&](unsigned r, u64 theirs, u64) {
-    if (r < row.rank) front += theirs;
-    mass += theirs;
-  });
+  const u64 mine[1] = {cta};
+  const u64(*all)[4] = row.exchange(mine);
+  for (unsigned r = 0; r < ranks; ++r) {
+    if (r < row.rank) front += all[r][0];
+    mass += all[r][0];
+  }
   const u64 target = target_of(mass);
   const u64 before = front + base + upto - local;
   const bool hit = before <= target && target < before + local;
@@ -775,7 +856,11 @@ int rl_sample_filtered(int dtype, const void* logits, int rows, int vocab, long 
   if (rows < 0 || rows > 65535 || vocab <= 0 || vocab > rl_sample_filtered_max_vocab() ||
       (temperature != nullptr && uniforms == nullptr && (seeds == nullptr || counters == nullptr)))
     return static_cast<int>(cudaErrorInvalidValue);
-  const int ranks = rl::filters::kMaxRanks;
+  // CTAs a row: as many as run at one time (two a multiprocessor), since a row's steps wait for one another more than they
+  // compute, and enough that a slice leaves room for two
+  const int slots = 2 * rl::filters::sm_count();
+  int ranks = rl::filters::kMaxRanks;
+  while (ranks > 1 && rows * ranks > slots && (vocab + ranks / 2 - 1) / (ranks / 2) <= rl::filters::kRoomySlice) ranks /= 2;
   rl::filters::Args a = {};
   a.logits = logits; a.row_stride = row_stride; a.vocab = vocab;
   a.slice = ((vocab + ranks - 1) / ranks + 7) & ~7;
@@ -794,8 +879,8 @@ int rl_sample_filtered(int dtype, const void* logits, int rows, int vocab, long 
   attributes[0].val.clusterDim.z = 1;
   attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attributes;
-  config.numAttrs = pdl ? 2 : 1;
+  config.attrs = ranks > 1 ? attributes : attributes + 1;      // a row in one CTA needs no cluster
+  config.numAttrs = (ranks > 1 ? 1 : 0) + (pdl ? 1 : 0);
   RL_DISPATCH_DTYPE(dtype, {
     static std::atomic<unsigned long long> configured;
     auto kernel = rl::filters::sample_filtered_kernel<scalar_t>;

@@ -250,37 +250,41 @@ class SharedItems(StepPlanner):
         """Rows of the two scratch buffers."""
         return plan["parts"] * self.group * self.num_kv_heads
 
-    # What an item takes, in units of a microsecond: a start (page ids, queries, the first keys, the result) and so much a block of 128
-    # keys; how many items of a kind a multiprocessor runs at one time.  By the kind of tile: rows of a tile -> (start, block, together).
-    COSTS = {256: (6.0, 2.4, 1), 128: (6.0, 1.3, 1), 64: (4.0, 1.2, 2), 32: (5.0, 5.0, 2), 16: (3.0, 1.0, 3)}
+    # Measured times in microseconds by the rows of a tile: an item's start (page ids, queries, first keys, result), a block of 128
+    # keys, and how many items a multiprocessor runs at one time; the join of the parts: its start, a part, a part of 1,024 rows.
+    COSTS = {256: (7.0, 1.7, 1), 128: (6.0, 0.95, 1), 64: (4.0, 1.2, 2), 32: (5.0, 5.0, 2), 16: (3.0, 0.9, 3)}
+    JOIN = (2.0, 0.05, 0.35)
+    STEPS = np.array([1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64, 96, 128, 192, 256, 512, 1024, 4096, 1 << 20])
 
-    def _blocks_per_item(self, tiles, rows, tile_rows: int) -> tuple[int, int]:
-        """Blocks of keys that a tile item and a row item take, for lists of (blocks, items side by side): so few that all
-        multiprocessors have work, and so many that the items, each with a start of its own and a part of its rows' results
-        to join, run at one time.  Of the steps tried the one whose longest item, or whose sum over the multiprocessors, is
-        done first."""
-        tile_start, tile_block, tile_together = self.COSTS[tile_rows]
-        row_start, row_block, row_together = self.COSTS[kernels.DECODE_TILE_ROWS]
-        longest = max([blocks for blocks, _ in [*tiles, *rows]] or [1])
-        steps = sorted({min(longest, step) for step in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 28, 32, 40, 48, 64, 96, 128, 192, 256, 512, 1024)})
-        best, chosen = None, (longest, longest)
-        row_steps = steps if rows else steps[:1]
-        for row_step in row_steps:
-            row_items = sum(-(-blocks // row_step) * side for blocks, side in rows)
-            row_time = sum(row_start * -(-blocks // row_step) * side + row_block * blocks * side for blocks, side in rows) / row_together
-            row_end = max([row_start + row_block * min(row_step, blocks) for blocks, _ in rows] or [0.0])
-            for step in steps if tiles else steps[:1]:
-                tile_items = sum(-(-blocks // step) * side for blocks, side in tiles)
-                tile_time = sum(tile_start * -(-blocks // step) * side + tile_block * blocks * side for blocks, side in tiles) / tile_together
-                tile_end = max([tile_start + tile_block * min(step, blocks) for blocks, _ in tiles] or [0.0])
-                waves = -(-tile_items // (self.sms * tile_together)) * tile_end
-                most_parts = max([-(-blocks // step) for blocks, _ in tiles] or [0]) + max([-(-blocks // row_step) for blocks, _ in rows] or [0])
-                end = max((row_time + tile_time) / self.sms, row_end, waves) + 0.15 * most_parts
-                if row_items > 60000 or tile_items > 60000:
-                    continue
-                if best is None or end < best - 1e-9:
-                    best, chosen = end, (step, row_step)
-        return chosen
+    def _blocks_per_item(self, tiles, rows, tile_rows: int, tokens: int) -> tuple[int, int]:
+        """Blocks of keys that a tile item and a row item take, for lists of (blocks, items side by side).  Short items fill the
+        multiprocessors, but each has a start of its own and leaves a part of its rows' results to join.  A tile has a multiprocessor
+        to itself (its threads hold every register), so row items run on those that are left, and behind the tiles.  Of the
+        steps tried, the pair whose estimated end comes first."""
+        def of(kind, costs):
+            start, block, together = costs
+            if not kind:
+                return np.array([1]), np.zeros(1), np.zeros(1), np.zeros(1), together
+            blocks, side = (np.array(column, dtype=np.int64) for column in zip(*kind))
+            steps = self.STEPS[: int(np.searchsorted(self.STEPS, int(blocks.max()))) + 1]
+            ranges = -(-blocks[None] // steps[:, None])
+            end = start + block * np.minimum(steps[:, None], blocks[None]).max(1)
+            return steps, (ranges * side).sum(1), end, ranges.max(1), together
+
+        tile_steps, tile_items, tile_end, tile_parts, tile_together = of(tiles, self.COSTS[tile_rows])
+        row_steps, row_items, row_end, row_parts, row_together = of(rows, self.COSTS[kernels.DECODE_TILE_ROWS])
+        tile_items, tile_end, tile_parts = tile_items[:, None], tile_end[:, None], tile_parts[:, None]
+        tile_slots, slots = self.sms * tile_together, self.sms * row_together
+        tiles_done = np.ceil(tile_items / tile_slots) * tile_end
+        left = np.maximum(self.sms - tile_items / tile_together, 0) * row_together
+        beside = left * np.where(row_end > 0, np.maximum(np.floor(tiles_done / np.maximum(row_end, 1e-9)), tile_items == 0), 0)
+        behind = np.ceil(np.maximum(row_items - beside, 0) / slots)
+        parts = tile_parts + row_parts
+        end = np.maximum(tiles_done, np.where(beside > 0, row_end, 0.0)) + behind * row_end
+        end = end + self.JOIN[0] + self.JOIN[1] * parts + self.JOIN[2] * parts * (tokens * self.group * self.num_kv_heads / 1024)
+        end = np.where((tile_items > 60000 * self.num_kv_heads) | (row_items > 60000 * self.num_kv_heads), np.inf, end)
+        at = np.unravel_index(int(np.argmin(end)), end.shape)
+        return int(tile_steps[at[0]]), int(row_steps[at[1]])
 
     def plan(self, shape: StepShape) -> dict:
         lengths, starts = np.asarray(shape.lengths, dtype=np.int64), np.asarray(shape.starts, dtype=np.int64)
@@ -323,12 +327,11 @@ class SharedItems(StepPlanner):
         def height_of(rows: int) -> int:
             return kernels.DECODE_TILE_ROWS if not self.wide and rows <= kernels.DECODE_TILE_ROWS else tile_rows
 
-        is_row = [not self.wide and rows <= kernels.DECODE_TILE_ROWS for rows in packed_rows]
-        tile_step, row_step = self._blocks_per_item(
-            [(-(-(end - first) // block), -(-rows // height_of(rows)) * self.num_kv_heads) for (_, first, end, _, _, _, _), rows, low
-             in zip(work, packed_rows, is_row) if not low],
-            [(-(-(end - first) // block), -(-rows // kernels.DECODE_TILE_ROWS) * self.num_kv_heads) for (_, first, end, _, _, _, _), rows, low
-             in zip(work, packed_rows, is_row) if low], tile_rows)
+        sides = {True: [], False: []}
+        for (_, first, end, _, _, _, _), packed in zip(work, packed_rows):
+            height = height_of(packed)
+            sides[height == kernels.DECODE_TILE_ROWS].append((-(-(end - first) // block), -(-packed // height) * self.num_kv_heads))
+        tile_step, row_step = self._blocks_per_item(sides[False], sides[True], tile_rows, tokens)
         parts = np.zeros(tokens, dtype=np.int64)                # of each token so far: a group's items come before its entries'
         tiles, rows, most = [], [], 0
         for entry, first, end, member, n, fresh, its in work:

@@ -117,6 +117,18 @@ def test_equal_logits(vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [300, 5000, 60000])
+def test_zeros_of_both_signs_are_equal(vocab):
+    x = torch.zeros((5, vocab), device=DEV)
+    x[:, torch.rand((vocab,), generator=torch.Generator(device=DEV).manual_seed(vocab), device=DEV) < 0.5] = -0.0
+    x[3, 7] = 1.0
+    for dtype in (torch.float32, torch.bfloat16):
+        for top_k, top_p in ((0, 0.5), (1, 1.0), (40, 0.5), (vocab // 2, 1.0), (vocab - 3, 0.9)):
+            run_case(x.to(dtype), 0.7, top_k, top_p, 0.0, draws(5))
+        run_case(x.to(dtype), 0.0, 0, 1.0, 0.0, draws(5))
+
+
+@pytest.mark.gpu
 def test_values_nearer_than_the_codes():
     """Thousands of different values within a tiny part of the row's range."""
     x = torch.full((4, 9000), -9.0, device=DEV)
