@@ -6,6 +6,7 @@ its own; every layer of a group uses the same page ids.  A request holds a *slot
 in every block table and in every per-request state tensor) and, per group, a list of
 pages.  Pages go back to the pool when the request ends, or, in a windowed or chunked group, as
 soon as the window or the chunk has passed them; they are handed out again to whoever asks next.
+Requests that were forked from one another hold the pages of their common tokens together.
 
 The reference keeps the same bookkeeping in ``BlockPool`` (null block 0, all-or-nothing
 ``get_new_blocks``, freed blocks reused first: ``rapid_llm/engine/block_pool.py:156-303``),
@@ -17,7 +18,7 @@ device (``rapid_llm/executor/slot_batch.py:130-178``); here tables hold page ids
 
 from __future__ import annotations
 
-from collections import deque
+from collections import Counter, deque
 from dataclasses import dataclass, field
 from typing import Hashable, Sequence
 
@@ -33,14 +34,15 @@ class CacheError(RuntimeError):
 
 
 class PagePool:
-    """Page ids ``1 .. num_pages``; id 0 is the null page and is never handed out."""
+    """Page ids ``1 .. num_pages``; id 0 is the null page and is never handed out.  A page has a number of holders: one after
+    :meth:`allocate`, one more for every :meth:`share`; it is free again when the last has given it back."""
 
     def __init__(self, num_pages: int) -> None:
         if num_pages < 1:
             raise ValueError(f"a pool needs at least one page, got {num_pages}")
         self.num_pages = num_pages
         self._free: deque[int] = deque(range(1, num_pages + 1))
-        self._held = [False] * (num_pages + 1)
+        self._holders = [0] * (num_pages + 1)
 
     @property
     def num_free(self) -> int:
@@ -58,25 +60,46 @@ class PagePool:
             return None
         pages = [self._free.popleft() for _ in range(count)]
         for page in pages:
-            if self._held[page]:
+            if self._holders[page]:
                 raise CacheError(f"page {page} was in the free list while held")
-            self._held[page] = True
+            self._holders[page] = 1
         return pages
 
+    def holders(self, page: int) -> int:
+        return self._holders[page]
+
+    def share(self, pages: Sequence[int]) -> None:
+        """One more holder for each of these held pages."""
+        real = [page for page in pages if page != NULL_PAGE]
+        for page in real:
+            if not 1 <= page <= self.num_pages or not self._holders[page]:
+                raise CacheError(f"page {page} is not held: it cannot be shared")
+        for page in real:
+            self._holders[page] += 1
+
+    def move(self, moves: Sequence[tuple[int, int]]) -> None:
+        """Held pages take the ids of free ones: ``(from, to)``, holders and all; what stays free is handed out from the lowest id on."""
+        for source, target in moves:
+            if not self._holders[source] or self._holders[target] or not 1 <= target <= self.num_pages:
+                raise CacheError(f"page {source} cannot move to {target}")
+            self._holders[target], self._holders[source] = self._holders[source], 0
+        self._free = deque(page for page in range(1, self.num_pages + 1) if not self._holders[page])
+
     def free(self, pages: Sequence[int]) -> None:
-        """Give pages back; they are the next to be handed out."""
+        """Give pages back; those whose last holder this was are the next to be handed out."""
         real = [page for page in pages if page != NULL_PAGE]
         for page in real:                       # check everything before anything changes
             if not 1 <= page <= self.num_pages:
                 raise CacheError(f"page {page} does not belong to this pool")
-            if not self._held[page]:
+            if not self._holders[page]:
                 raise CacheError(f"page {page} freed twice")
         if len(set(real)) != len(real):
             raise CacheError("a page is named twice in one free")
         for page in real:
-            self._held[page] = False
+            self._holders[page] -= 1
         for page in reversed(real):
-            self._free.appendleft(page)
+            if not self._holders[page]:
+                self._free.appendleft(page)
 
     def check(self) -> None:
         """Raise unless every page is exactly once either free or held."""
@@ -84,9 +107,9 @@ class PagePool:
         if len(set(free)) != len(free):
             raise CacheError("a page is in the free list twice")
         for page in free:
-            if self._held[page]:
+            if self._holders[page]:
                 raise CacheError(f"page {page} is both free and held")
-        if len(free) + sum(self._held[1:]) != self.num_pages:
+        if len(free) + sum(1 for holders in self._holders[1:] if holders) != self.num_pages:
             raise CacheError("a page was lost")
 
 
@@ -146,6 +169,7 @@ class _Held:
     slot: int
     num_tokens: int = 0                      # tokens whose K/V are (being) cached
     pages: list[list[int]] = field(default_factory=list)   # per group, NULL_PAGE where released
+    family: tuple[int, int] | None = None    # requests forked from one another: their number, and the positions whose pages all share
 
 
 class CacheManager:
@@ -182,6 +206,7 @@ class CacheManager:
         ]
         self._free_slots = list(range(self.max_num_seqs - 1, -1, -1))
         self._held: dict[Hashable, _Held] = {}
+        self._families = 0
         self.dirty_slots: list[set[int]] = [set() for _ in self.groups]
 
     # -- queries ------------------------------------------------------------------ #
@@ -292,6 +317,64 @@ class CacheManager:
                 self.dirty_slots[index].add(held.slot)
         self._free_slots.append(held.slot)
 
+    # -- several requests behind the same tokens -------------------------------------- #
+    def fork(self, parent: Hashable, children: Sequence[Hashable]) -> list[list[tuple[int, int]]] | None:
+        """Admit ``children`` as continuations of ``parent`` from where it is: the same tokens are cached, the pages they fill are
+        shared (no one writes into those again), and each child gets a page of its own for the ragged last one.  Returns, per
+        group, the ``(page of the parent, page of a child)`` copies that the device has to make before anyone writes on; ``None``
+        (and nothing taken) when slots or pages are short."""
+        held = self._get(parent)
+        children = list(children)
+        if len(set(children)) != len(children) or any(child in self._held for child in children):
+            raise CacheError("a child is named twice or already admitted")
+        if len(children) > len(self._free_slots):
+            return None
+        whole, ragged = divmod(held.num_tokens, self.page_size)
+        copied = [bool(ragged) and pages[whole] != NULL_PAGE for pages in held.pages]
+        if any(copy and len(children) > pool.num_free for copy, pool in zip(copied, self.pools)):
+            return None
+        if whole and held.family is None and children:
+            self._families += 1
+            held.family = (self._families, whole * self.page_size)
+        copies: list[list[tuple[int, int]]] = [[] for _ in self.groups]
+        for child in children:
+            slot = self.admit(child)
+            assert slot is not None
+            its = self._held[child]
+            its.num_tokens, its.family = held.num_tokens, held.family
+            for index, pages in enumerate(held.pages):
+                its.pages[index] = pages[:whole]
+                self.pools[index].share(its.pages[index])
+                if ragged:
+                    its.pages[index].append(NULL_PAGE)
+                    if copied[index]:
+                        its.pages[index][whole] = self.pools[index].allocate(1)[0]
+                        copies[index].append((pages[whole], its.pages[index][whole]))
+                self.block_tables[index][slot, : len(its.pages[index])] = its.pages[index]
+                self.dirty_slots[index].add(slot)
+        return copies
+
+    def shared_prefix(self, request_id: Hashable) -> tuple[int, int] | None:
+        """Number of the request's family and the positions whose pages it shares with every other of it, if it has one."""
+        return self._get(request_id).family
+
+    def compact(self, group: int) -> list[tuple[int, int]]:
+        """Move a group's held pages to the lowest ids; the ``(from, to)`` copies that the device has to make."""
+        pool = self.pools[group]
+        held = pool.num_held
+        sources = [page for page in range(held + 1, pool.num_pages + 1) if pool.holders(page)]
+        targets = [page for page in range(1, held + 1) if not pool.holders(page)]
+        moves = list(zip(sources, targets))
+        pool.move(moves)
+        new = dict(moves)
+        for its in self._held.values():
+            pages = its.pages[group]
+            if any(page in new for page in pages):
+                pages[:] = [new.get(page, page) for page in pages]
+                self.block_tables[group][its.slot, : len(pages)] = pages
+                self.dirty_slots[group].add(its.slot)
+        return moves
+
     # -- per-step views ------------------------------------------------------------ #
     def kv_destinations(self, group: int, slot: int, start: int, count: int) -> np.ndarray:
         """``page * page_size + offset`` for positions ``start .. start + count - 1``."""
@@ -305,17 +388,18 @@ class CacheManager:
         return slots
 
     def check(self) -> None:
-        """Raise unless no page is lost, held twice or both held and free."""
+        """Raise unless no page is lost, has other holders than its pool counts, or is both held and free."""
         for index, pool in enumerate(self.pools):
             pool.check()
             owned: list[int] = []
             for held in self._held.values():
                 owned.extend(page for page in held.pages[index] if page != NULL_PAGE)
-            if len(set(owned)) != len(owned):
-                raise CacheError(f"group {index}: a page is held by two requests")
-            if len(owned) != pool.num_held:
+            counted = Counter(owned)
+            if any(pool.holders(page) != count for page, count in counted.items()):
+                raise CacheError(f"group {index}: a page is held by another number of requests than its pool counts")
+            if len(counted) != pool.num_held:
                 raise CacheError(
-                    f"group {index}: requests hold {len(owned)} pages, the pool says {pool.num_held}"
+                    f"group {index}: requests hold {len(counted)} pages, the pool says {pool.num_held}"
                 )
         slots = [held.slot for held in self._held.values()]
         if len(set(slots)) != len(slots) or set(slots) & set(self._free_slots):

@@ -16,8 +16,9 @@ from typing import Sequence
 
 import torch
 
+from ..ops import kernels
 from ..parts.base import StateNeed
-from .manager import CacheManager
+from .manager import NULL_PAGE, CacheError, CacheManager
 
 
 class CacheStorage:
@@ -63,6 +64,18 @@ class CacheStorage:
         for state in self.states:
             if state is not None:
                 state[slot].zero_()
+
+    def copy_pages(self, group: int, pairs: Sequence[tuple[int, int]]) -> None:
+        """Copy pages of one group, in every layer of it; the null page is never written."""
+        if any(target == NULL_PAGE for _, target in pairs):
+            raise CacheError("the null page is not written")
+        kernels.copy_pages(self.pages[group], pairs)
+
+    def copy_state(self, source: int, targets: Sequence[int]) -> None:
+        """The per-request states of slot ``source`` into the slots ``targets``."""
+        for state in self.states:
+            if state is not None and state.numel():
+                kernels.copy_pages(state.unsqueeze(0), [(source, target) for target in targets])
 
     def nbytes(self) -> int:
         total = sum(p.numel() * p.element_size() for p in self.pages)

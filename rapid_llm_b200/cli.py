@@ -39,6 +39,9 @@ def _add_engine_options(sub: argparse.ArgumentParser) -> None:
     sub.add_argument("--device", default="cuda")
     sub.add_argument("--temperature", type=float, default=0.6)
     sub.add_argument("--top-p", type=float, default=0.9)
+    sub.add_argument("--top-k", type=int, default=0, help="keep the k largest logits before top-p; 0 = all")
+    sub.add_argument("--min-p", type=float, default=0.0, help="keep what has at least this share of the largest probability")
+    sub.add_argument("--n", type=int, default=1, help="completions per prompt, from one computation of it")
     sub.add_argument("--max-gen-len", type=int, default=None)
     sub.add_argument("--repetition-penalty", type=float, default=1.1,
                      help="Penalise logits of already-generated tokens (1.0 disables it)")
@@ -72,7 +75,7 @@ def _sampling(args):
 
     return SamplingParams(
         temperature=args.temperature, top_p=args.top_p, max_gen_len=args.max_gen_len,
-        repetition_penalty=args.repetition_penalty, seed=args.seed,
+        repetition_penalty=args.repetition_penalty, seed=args.seed, top_k=args.top_k, min_p=args.min_p, n=args.n,
     )
 
 
@@ -124,12 +127,13 @@ def _build_llm(args):
 
 def _report(args, outputs, started: float, elapsed: float) -> int:
     for index, output in enumerate(outputs):
-        completion = output.outputs[0]
-        print(f"--- [{index}] {completion.finish_reason} ---")
-        print(completion.text.strip() if completion.text else " ".join(map(str, completion.token_ids)))
-        print()
+        for completion in output.outputs:
+            place = str(index) if len(output.outputs) == 1 else f"{index}.{completion.index}"
+            print(f"--- [{place}] {completion.finish_reason} ---")
+            print(completion.text.strip() if completion.text else " ".join(map(str, completion.token_ids)))
+            print()
     if args.show_stats:
-        generated = sum(len(o.outputs[0].token_ids) for o in outputs)
+        generated = sum(len(completion.token_ids) for o in outputs for completion in o.outputs)
         ttfts = [(o.metrics["first_token"] - started) * 1000 for o in outputs if o.metrics.get("first_token")]
         print(f"{len(outputs)} requests, {generated} tokens in {elapsed:.2f}s")
         print(f"throughput {generated / elapsed:7.1f} tok/s")

@@ -766,9 +766,11 @@ static int launch_decode_tc(const AttentionArgs& a, int n_items, int max_rows, b
   return launch_decode_tc_rows<16>(map, t, n_items, pdl, stream, g_decode_tc_configured[4], rings);
 }
 
-// Listed items of up to 16 packed rows: from memory straight into the tensor cores' registers (heads of 64 and 128).
+// Listed items of up to 16 packed rows: from memory straight into the tensor cores' registers (heads of 64 and 128; a
+// template, so that the others' builds do without these kernels).
+template <int kDim>
 static int launch_rows(const AttentionArgs& a, int n_items, int most_rows, bool early, bool pdl, cudaStream_t stream) {
-  if constexpr (!kRwTakes) {
+  if constexpr (kDim != 64 && kDim != 128) {
     return static_cast<int>(cudaErrorInvalidValue);
   } else {
     RowsArgs t = {};
@@ -793,7 +795,11 @@ static int launch_shared_tc_as(const CUtensorMap& map, const SharedTcArgs& t, in
   return launch_kernel(kernel, dim3(t.hkv, n_items), dim3(kShThreads), sh_smem_bytes(kTwoTiles), stream, pdl, map, t);
 }
 
+template <int kDim>
 static int launch_shared_tc(const AttentionArgs& a, int n_items, int tile_rows, bool pdl, cudaStream_t stream) {
+  if constexpr (kDim != kTcD) {
+    return static_cast<int>(cudaErrorInvalidValue);
+  } else {
   CUtensorMap map;
   const long long rows = static_cast<long long>(a.num_pages) * 2 * a.hkv * a.page_size;
   int status = make_map(&map, a.cache, rows, kD, a.page_size < kShKeys ? a.page_size : kShKeys);
@@ -808,6 +814,7 @@ static int launch_shared_tc(const AttentionArgs& a, int n_items, int tile_rows, 
                                : launch_shared_tc_as<true, false>(map, t, n_items, pdl, stream);
   return a.slopes != nullptr ? launch_shared_tc_as<false, true>(map, t, n_items, pdl, stream)
                              : launch_shared_tc_as<false, false>(map, t, n_items, pdl, stream);
+  }
 }
 
 }  // namespace RL_ATTENTION_NS
@@ -990,14 +997,10 @@ int rl_attention_shared(const void* q, const void* cache, void* out, float* part
   args.members = members; args.positions = positions; args.part_first = part_first;
   args.fault = fault;
   int status = 0;
-  if constexpr (attn::kD == attn::kTcD) {
-    if (tile_rows != 64) {
-      if (n_tile_items > 0) {
-        args.items = tile_items;
-        status = attn::launch_shared_tc(args, n_tile_items, tile_rows, pdl != 0, stream);
-        if (status != 0) return status;
-      }
-    }
+  if (tile_rows != 64 && n_tile_items > 0) {
+    args.items = tile_items;
+    status = attn::launch_shared_tc<attn::kD>(args, n_tile_items, tile_rows, pdl != 0, stream);
+    if (status != 0) return status;
   }
   if (tile_rows == 64 && n_tile_items > 0) {
     args.items = tile_items;
@@ -1009,7 +1012,7 @@ int rl_attention_shared(const void* q, const void* cache, void* out, float* part
     args.items = row_items;
     const bool dependent = n_tile_items > 0 || pdl != 0;
     if (attn::kRwTakes) {
-      status = attn::launch_rows(args, n_row_items, most_rows, n_tile_items > 0, dependent, stream);
+      status = attn::launch_rows<attn::kD>(args, n_row_items, most_rows, n_tile_items > 0, dependent, stream);
     } else {
       status = slopes != nullptr ? attn::launch_attention_as<1, 4, 3, false, true, true>(args, n_row_items, dependent, stream)
                                  : attn::launch_attention_as<1, 4, 3, false, false, true>(args, n_row_items, dependent, stream);

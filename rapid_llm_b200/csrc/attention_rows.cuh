@@ -21,7 +21,7 @@
 namespace rl {
 namespace RL_ATTENTION_NS {
 
-constexpr bool kRwTakes = kD == 64 || kD == 128;
+constexpr bool kRwTakes = kD == 64 || kD == 128;     // (the kernel is built for these alone)
 constexpr int kRwWarps = 4;
 constexpr int kRwKeys = 16;                    // keys of a step
 constexpr int kRwStagedPages = 512;

@@ -434,6 +434,8 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   row.chunk = ((row.count + kThreads - 1) / kThreads) | 1;      // odd: a warp's lanes then read different banks
   for (int j = threadIdx.x; j < 64; j += kThreads) s.table[j] = exp2(static_cast<double>(j) / 64.0);
   pdl_wait();
+  const int want_k = args.top_k ? args.top_k[row_index] : 0;
+  if (want_k < 0) return;                            // the whole cluster: this row's place in `out` stays as it is
   const float temp = args.temperature ? args.temperature[row_index] : 0.0f;
   const float pen = args.penalty ? args.penalty[row_index] : 1.0f;
   const int seen_begin = args.seen_offsets ? args.seen_offsets[row_index] : 0;
@@ -522,7 +524,6 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   }
   constexpr unsigned kLast = (1u << kCodeBits) - 1u;
 
-  const int want_k = args.top_k ? args.top_k[row_index] : 0;
   const float p = args.top_p ? args.top_p[row_index] : 1.0f;
   const float least_p = args.min_p ? fminf(args.min_p[row_index], 1.0f) : 0.0f;
   const double least_weight = static_cast<double>(least_p) * kUnit;

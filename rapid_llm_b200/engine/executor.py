@@ -26,6 +26,9 @@ class DeviceExecutor:
     def release(self, request_id: Hashable) -> None:
         self.runner.release(request_id)
 
+    def fork(self, parent: Hashable, children: Sequence[Hashable]) -> bool:
+        return self.runner.fork(parent, children)
+
     def launch(self, entries: Sequence):
         """Enqueue the batch, its sampling and the read of the sampled ids; returns a ticket.
 

@@ -160,7 +160,8 @@ class LLM:
                 requests.append(self.scheduler.add_request(ids, params))
         except Exception:
             for request in requests:          # a refused prompt takes the call's earlier ones with it
-                self.scheduler.abort(request)
+                for completion in request.completions:
+                    self.scheduler.abort(completion)
             raise
         return encoded, requests
 
@@ -170,6 +171,9 @@ class LLM:
         the list of new token ids (``rapid_llm/engine/llm.py:197-222`` yields text pieces the
         same way).  Tokens that are still only on the device (the scheduler runs a step ahead)
         are reported once the host has read them."""
+        sets = [sampling_params] if isinstance(sampling_params, SamplingParams) else list(sampling_params or ())
+        if any(params.n > 1 for params in sets):
+            raise ValueError("stream yields one completion per prompt: n must be 1 (generate takes more)")
         _, requests = self._submit(prompts, sampling_params)
         reported = [0] * len(requests)
         texts = [""] * len(requests)
@@ -197,17 +201,21 @@ class LLM:
         """Generate for every prompt; returns one ``RequestOutput`` per prompt, in order.
 
         ``prompts``: a string, a list of strings, one list of token ids, or a list of them.
-        ``sampling_params``: one set for all prompts, or one per prompt.
+        ``sampling_params``: one set for all prompts, or one per prompt; ``n`` of them gives that many completions in
+        ``RequestOutput.outputs``, drawn from one computation of the prompt.
         """
         encoded, requests = self._submit(prompts, sampling_params)
         self.scheduler.run_to_completion()
         outputs = []
         for (text, ids), request in zip(encoded, requests):
-            completion = CompletionOutput(0, self._decode(request.output_token_ids), list(request.output_token_ids), request.finish_reason)
+            completions = [
+                CompletionOutput(index, self._decode(each.output_token_ids), list(each.output_token_ids), each.finish_reason)
+                for index, each in enumerate(request.completions)
+            ]
             metrics = {
                 "arrival": request.arrival_time, "first_scheduled": request.first_scheduled_time,
                 "first_token": request.first_token_time, "finished": request.finish_time,
                 "preemptions": request.num_preemptions,
             }
-            outputs.append(RequestOutput(text, ids, [completion], metrics))
+            outputs.append(RequestOutput(text, ids, completions, metrics))
         return outputs

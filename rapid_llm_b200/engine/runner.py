@@ -13,6 +13,7 @@ workspace and the per-step metadata upload (one pinned buffer, one copy).
 
 from __future__ import annotations
 
+from collections import Counter
 from dataclasses import dataclass
 from pathlib import Path
 from typing import Any, Hashable, Mapping, Sequence
@@ -181,6 +182,31 @@ class ModelRunner:
     def release(self, request_id: Hashable) -> None:
         self.cache.release(request_id)
 
+    def fork(self, parent: Hashable, children: Sequence[Hashable]) -> bool:
+        """Admit ``children`` as continuations of ``parent`` from where it is: they have cached what it has, share its whole pages
+        and start with copies of its ragged last page and of its per-request states.  ``False`` (and nothing done) when slots or
+        pages are short.  Decode steps then read what a family shares once, where that is worth it."""
+        copies = self.cache.fork(parent, children)
+        if copies is None:
+            return False
+        for group, pairs in enumerate(copies):
+            if pairs:
+                self.storage.copy_pages(group, pairs)
+        if children:
+            self.storage.copy_state(self.cache.slot_of(parent), [self.cache.slot_of(child) for child in children])
+        return True
+
+    def compact(self) -> int:
+        """Move every group's held pages to the lowest ids (steps that are enqueued keep theirs: the copies run behind
+        them); returns how many pages moved."""
+        moved = 0
+        for group in range(len(self.cache.groups)):
+            pairs = self.cache.compact(group)
+            if pairs:
+                self.storage.copy_pages(group, pairs)
+            moved += len(pairs)
+        return moved
+
     def num_cached_tokens(self, request_id: Hashable) -> int:
         return self.cache.num_tokens(request_id)
 
@@ -256,6 +282,7 @@ class ModelRunner:
             decode_only=max(lengths) == 1,
             page_size=cache.page_size,
             padding=pad,
+            **self._prefixes(entries, pad),
         )
         planned: dict[tuple, dict[str, Any]] = {}
         for planner in self._planners:
@@ -358,6 +385,20 @@ class ModelRunner:
             extras=extras,
             feedback=self.result[1:],
         )
+
+    def _prefixes(self, entries: Sequence[StepEntry], pad: int) -> dict[str, np.ndarray]:
+        """Which of the step's entries share the pages of how many first positions (nothing if none do)."""
+        families = [self.cache.shared_prefix(entry.request_id) for entry in entries]
+        if not any(families):
+            return {}
+        together = Counter(family[0] for family in families if family is not None)
+        shares = [family is not None and together[family[0]] > 1 for family in families]
+        if not any(shares):
+            return {}
+        return {
+            "prefix_group": np.asarray([family[0] if use else -1 for family, use in zip(families, shares)] + [-1] * pad, dtype=np.int32),
+            "prefix_tokens": np.asarray([family[1] if use else 0 for family, use in zip(families, shares)] + [0] * pad, dtype=np.int32),
+        }
 
     def layer_caches(self) -> list[LayerCache]:
         caches = []

@@ -23,6 +23,11 @@ when the scheduler was given a detokenizer, ``"repeat"``: every eighth step the 
 with ``stop_on_repeat`` is checked for a loop (``engine/repetition.py``), as the reference does
 (``rapid_llm/engine/scheduler.py:1398-1455``).
 
+Several completions of one prompt (``SamplingParams.n``): the first of them computes the prompt, its last token left out;
+there the others are forked from it (they share its pages, see ``CacheManager.fork``), and all of them feed that token side by
+side and sample on their own.  Those that find no slot or page then, and those whose prompt has one token, compute the
+prompt themselves, like requests of their own.
+
 Running ahead.  A step's sampled tokens stay on the device, where the next step's embedding
 can pick them up, so the next step can be planned and enqueued before the host has seen them:
 everything else a step needs (positions, pages, which rows to sample) follows from counts.
@@ -52,6 +57,8 @@ from .repetition import CHECK_EVERY, text_repeats
 
 WAITING, RUNNING, FINISHED = "waiting", "running", "finished"
 
+SEED_STRIDE = 0x9E3779B97F4A7C15      # odd: the completions of one request draw from different streams
+
 
 class CacheExhausted(RuntimeError):
     """No running request can make progress and eviction is off."""
@@ -76,6 +83,7 @@ class Request:
     first_scheduled_time: float | None = None
     first_token_time: float | None = None
     finish_time: float | None = None
+    completions: list["Request"] = field(default_factory=list)      # of a request with n > 1: itself and the n - 1 others
 
     @property
     def all_token_ids(self) -> list[int]:
@@ -150,6 +158,7 @@ class Scheduler:
         self.waiting: deque[Request] = deque()
         self.running: list[Request] = []      # in admission order: the last is the youngest
         self._ids = itertools.count()
+        self._to_fork: dict[Hashable, list[Request]] = {}      # by the request that computes their prompt
         self.num_steps = 0
         self.num_preemptions = 0
         self._inflight: Inflight | None = None
@@ -218,16 +227,27 @@ class Scheduler:
         seed = params.seed if params.seed is not None else zlib.crc32(repr(request_id).encode())
         request = Request(request_id, prompt, params, max_new, seed, arrival_time=time.perf_counter())
         self.waiting.append(request)
+        others = [
+            Request((request_id, index), prompt, params, max_new, (seed + index * SEED_STRIDE) % 2**63, arrival_time=request.arrival_time)
+            for index in range(1, params.n)
+        ]
+        request.completions = [request, *others]
+        if others and len(prompt) > 1 and hasattr(self.executor, "fork"):
+            self._to_fork[request_id] = others
+        else:
+            self.waiting.extend(others)
         return request
 
     def has_unfinished(self) -> bool:
-        return bool(self.waiting or self.running or self._inflight is not None)
+        return bool(self.waiting or self.running or self._to_fork or self._inflight is not None)
 
     has_unfinished_requests = has_unfinished      # the reference's name
 
     # -- planning -------------------------------------------------------------------- #
     def _chunk(self, request: Request, budget: int) -> int:
         remaining = request.num_tokens - request.num_computed_tokens
+        if request.request_id in self._to_fork:
+            remaining -= 1                        # the others are forked before the prompt's last token
         if self.config.enable_chunked_prefill:
             return min(remaining, self.config.max_chunk_size, budget)
         return remaining if remaining <= budget else 0
@@ -256,7 +276,25 @@ class Scheduler:
         self.waiting.appendleft(victim)
         plan.preempted.append(victim)
 
+    def _fork(self) -> None:
+        """Fork the others of every request that has computed its prompt but for the last token."""
+        for request in [r for r in self.running if r.request_id in self._to_fork]:
+            if request.num_computed_tokens != len(request.prompt_token_ids) - 1:
+                continue
+            others = self._to_fork.pop(request.request_id)
+            fitting = others[: max(min(self.config.max_num_seqs - len(self.running), self.cache.num_free_slots), 0)]
+            while fitting and not self.executor.fork(request.request_id, [other.request_id for other in fitting]):
+                fitting = fitting[:-1]            # pages are short: fewer of them
+            place = self.running.index(request) + 1
+            for other in fitting:
+                other.status = RUNNING
+                other.num_computed_tokens = request.num_computed_tokens
+                other.first_scheduled_time = time.perf_counter()
+            self.running[place:place] = fitting
+            self.waiting.extendleft(reversed(others[len(fitting) :]))
+
     def plan(self) -> StepPlan:
+        self._fork()
         plan = StepPlan()
         budget = self.config.max_num_batched_tokens
         free = [pool.num_free for pool in self.cache.pools]
@@ -416,11 +454,18 @@ class Scheduler:
             self.executor.release(request.request_id)
         elif request in self.waiting:                    # evicted while its last token was in flight
             self.waiting.remove(request)
+        else:
+            for others in self._to_fork.values():        # not forked yet
+                if request in others:
+                    others.remove(request)
+        self.waiting.extendleft(reversed(self._to_fork.pop(request.request_id, [])))      # no one computes their prompt any more
+        self._to_fork = {leader: others for leader, others in self._to_fork.items() if others}
 
     def abort(self, request: Request | Hashable) -> None:
         """End a request now; takes the handle or, as the reference does, its id."""
         if not isinstance(request, Request):
-            request = next((r for r in [*self.running, *self.waiting] if r.request_id == request), None)
+            unforked = itertools.chain.from_iterable(self._to_fork.values())
+            request = next((r for r in [*self.running, *self.waiting, *unforked] if r.request_id == request), None)
             if request is None:
                 return
         if request.status in (RUNNING, WAITING):

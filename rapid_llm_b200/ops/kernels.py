@@ -173,6 +173,8 @@ def core() -> ctypes.CDLL:
             "rl_qk_norm_rope_write", "rl_attention_generic", "rl_attention_shared_f32", "rl_copy_pages", "rl_copy_pages_launches", "rl_gemm_f32", "rl_sample",
         ):
             getattr(lib, name).restype = c_int
+        if lib.rl_attention_shared_f32_rows() != SHARED_F32_ROWS:
+            raise KernelError("the float32 kernel over shared prefixes was built for other tiles than the host's")
         _SIGNATURES_SET = True
     return lib
 
@@ -1256,7 +1258,8 @@ def sample(
     ``counters``) given, a row keeps its ``top_k`` largest logits (of equal ones those of lowest index), of those what has
     at most ``top_p`` of their mass strictly above it, and of those what has at least ``min_p`` of the largest
     probability; the draw is the first index whose running kept mass exceeds ``u`` of all kept mass.  Masses are exact to 2^-43 of the
-    largest weight.  A row with ``temperature`` 0 takes the first maximum.  Every array has one entry a row."""
+    largest weight.  A row with ``temperature`` 0 takes the first maximum; one with ``top_k`` below 0 is passed over, its place in
+    ``out`` stays as it is.  Every array has one entry a row."""
     _need_cuda(logits, out, temperature, top_p, penalty, seeds, counters, seen_tokens, seen_offsets, top_k, min_p, uniforms)
     _expect("out", out, torch.int32)
     for name, tensor in (("temperature", temperature), ("top_p", top_p), ("penalty", penalty), ("min_p", min_p), ("uniforms", uniforms)):

@@ -114,7 +114,8 @@ class AttentionItems(StepPlanner):
 
     def __init__(self, group: int, num_kv_heads: int, head_dim: int = 0, sms: int = DEFAULT_SMS,
                  decode_clusters: dict[int, int] | None = None, tensor_core: bool = True,
-                 decode_tensor_core: bool = True, chunk: int = 0, window: int = 0, one_plane: bool = False) -> None:
+                 decode_tensor_core: bool = True, chunk: int = 0, window: int = 0, one_plane: bool = False,
+                 shared: SharedItems | None = None) -> None:
         self.group, self.num_kv_heads, self.head_dim = int(group), int(num_kv_heads), int(head_dim)
         # decode_tensor_core False: the mixer's scores are squashed, which the tcgen05 chunk tiles and the mma.sync tiles
         # compute, the tcgen05 decode tiles not; tensor_core False: mma.sync tiles only.  chunk: the most keys a
@@ -127,20 +128,30 @@ class AttentionItems(StepPlanner):
         self.plane_decode_tiles = int(sms)
         # window: the same bound for the key ranges where a mixer asks for it (0 = not bounded).
         self.chunk, self.window = int(chunk), int(window)
+        # shared: cuts the decode steps whose requests share prefixes worth reading once (the plan then says "shared")
+        self.shared = shared
         self.decode_clusters = dict(decode_clusters or DEFAULT_DECODE_CLUSTERS)
         # work items the kernels want in flight: two CTAs per multiprocessor, one in a decode-only
         # step, whose kernel keeps a whole multiprocessor's shared memory busy
         self.target_ctas, self.decode_target_ctas = 2 * int(sms), int(sms)
         self.key = ("attention_items", self.group, self.num_kv_heads, self.head_dim, int(sms),
                     tuple(sorted(self.decode_clusters.items())), self.tensor_core, self.decode_tensor_core, self.chunk, self.window,
-                    self.one_plane)
+                    self.one_plane) + (() if shared is None else (shared.key,))
 
     def capacity(self, max_tokens: int, max_entries: int) -> int:
+        own = self._own_capacity(max_tokens, max_entries)
+        return own if self.shared is None else max(own, self.shared.capacity(max_tokens, max_entries))
+
+    def _own_capacity(self, max_tokens: int, max_entries: int) -> int:
         chunk_tiles = -(-max_tokens * self.group // kernels.CHUNK_TILE_ROWS) + max_entries
         decode_tiles = max_entries * -(-self.group // kernels.DECODE_TILE_ROWS)
         return 4 * (chunk_tiles + decode_tiles + 2 * self.target_ctas)
 
     def plan(self, shape: StepShape) -> dict:
+        if self.shared is not None and shape.prefix_group is not None:
+            shared = self.shared.step_plan(shape)
+            if shared is not None:
+                return shared
         lengths = np.asarray(shape.lengths, dtype=np.int64)
         starts = np.asarray(shape.starts, dtype=np.int64)
         rows = lengths * self.group
@@ -263,9 +274,9 @@ class SharedItems(StepPlanner):
         steps tried, the pair whose estimated end comes first."""
         def of(kind, costs):
             start, block, together = costs
-            if not kind:
+            if len(kind) == 0:
                 return np.array([1]), np.zeros(1), np.zeros(1), np.zeros(1), together
-            blocks, side = (np.array(column, dtype=np.int64) for column in zip(*kind))
+            blocks, side = np.asarray(kind)[:, 0], np.asarray(kind)[:, 1]
             steps = self.STEPS[: int(np.searchsorted(self.STEPS, int(blocks.max()))) + 1]
             ranges = -(-blocks[None] // steps[:, None])
             end = start + block * np.minimum(steps[:, None], blocks[None]).max(1)
@@ -298,67 +309,110 @@ class SharedItems(StepPlanner):
             raise ValueError("shared positions must lie before an entry's new tokens")
         first_token = np.concatenate(([0], np.cumsum(lengths)))
         tokens = int(first_token[-1])
-        members = [np.arange(tokens, dtype=np.int64)]           # an entry's own rows, then each group's
-        at = tokens
-        block = kernels.DECODE_TC_KEYS
-        work = []                                               # entry, first key, end, first member, rows, fresh key, tokens
+        entry_of = np.repeat(np.arange(count), lengths)
+        # Columns: entry, first key, end, first member, packed rows, fresh key, parts of its tokens before it.  The members are the step's
+        # tokens, for an entry's own keys, and behind them each group's.
+        members, at, work = [np.arange(tokens, dtype=np.int64)], tokens, []
         for number in np.unique(groups[(groups >= 0) & (shared > 0)]):
             inside = np.flatnonzero(groups == number)
-            if (shared[inside] != shared[inside[0]]).any():
-                raise ValueError("the entries of a group share one number of positions")
-            its = np.concatenate([np.arange(first_token[e], first_token[e + 1]) for e in inside])
-            members.append(its)
             keys = int(shared[inside[0]])
-            work.append((int(inside[0]), 0, keys, at, len(its), keys, its))
+            if (shared[inside] != keys).any():
+                raise ValueError("the entries of a group share one number of positions")
+            its = np.flatnonzero(groups[entry_of] == number)
+            members.append(its)
+            work.append((int(inside[0]), 0, keys, at, len(its) * self.group, keys, 0))
             at += len(its)
-        for entry in range(count):
-            its = np.arange(first_token[entry], first_token[entry + 1])
-            work.append((entry, int(shared[entry]), int(starts[entry] + lengths[entry]), int(first_token[entry]), len(its),
-                         int(starts[entry]), its))
-
-        packed_rows = [n * self.group for _, _, _, _, n, _, _ in work]
+        prefixes = np.array(work, dtype=np.int64).reshape(-1, 7)
+        own = np.stack([np.arange(count), shared, starts + lengths, first_token[:-1], lengths * self.group, starts, np.zeros(count, dtype=np.int64)], 1)
+        work = np.concatenate([prefixes, own])
+        low = (work[:, 4] <= kernels.DECODE_TILE_ROWS) & (not self.wide)
         if self.wide:
             tile_rows = kernels.SHARED_F32_ROWS
         elif not kernels.attention_tc_takes(self.head_dim, shape.page_size):
             tile_rows = kernels.CHUNK_TILE_ROWS
         else:
-            tile_rows = kernels.SHARED_TC_ROWS[max(packed_rows) > kernels.SHARED_TC_ROWS[0]]
+            tile_rows = kernels.SHARED_TC_ROWS[int(work[:, 4].max()) > kernels.SHARED_TC_ROWS[0]]
+        height = np.where(low, kernels.DECODE_TILE_ROWS, tile_rows)
+        block = kernels.DECODE_TC_KEYS
+        blocks, high = -(-(work[:, 2] - work[:, 1]) // block), -(-work[:, 4] // height)
+        tile_step, row_step = self._blocks_per_item(np.stack([blocks, high * self.num_kv_heads], 1)[~low],
+                                                    np.stack([blocks, high * self.num_kv_heads], 1)[low], tile_rows, tokens)
+        # key ranges of equal length, in whole blocks
+        ranges = -(-blocks // np.where(low, row_step, tile_step))
+        step = -(-blocks // ranges) * block
+        ranges = -(-(work[:, 2] - work[:, 1]) // step)
+        everyone = np.concatenate(members)
+        parts = ranges[len(prefixes) :][entry_of]
+        for (_, _, _, first, rows, _, _), used in zip(prefixes, ranges):
+            its = everyone[first : first + rows // self.group]
+            parts[its] += used
+            work[len(prefixes) + entry_of[its], 6] = used
 
-        def height_of(rows: int) -> int:
-            return kernels.DECODE_TILE_ROWS if not self.wide and rows <= kernels.DECODE_TILE_ROWS else tile_rows
-
-        sides = {True: [], False: []}
-        for (_, first, end, _, _, _, _), packed in zip(work, packed_rows):
-            height = height_of(packed)
-            sides[height == kernels.DECODE_TILE_ROWS].append((-(-(end - first) // block), -(-packed // height) * self.num_kv_heads))
-        tile_step, row_step = self._blocks_per_item(sides[False], sides[True], tile_rows, tokens)
-        parts = np.zeros(tokens, dtype=np.int64)                # of each token so far: a group's items come before its entries'
-        tiles, rows, most = [], [], 0
-        for entry, first, end, member, n, fresh, its in work:
-            packed = n * self.group
-            height = height_of(packed)
-            low_item = not self.wide and packed <= kernels.DECODE_TILE_ROWS
-            bucket, per_item = (rows, row_step) if low_item else (tiles, tile_step)
-            if bucket is rows:
-                most = max(most, min(height, packed))
-            ranges = max(1, -(-(end - first) // (per_item * block)))
-            step = -(-(-(-(end - first) // ranges)) // block) * block
-            lows = range(first, end, step)
-            offset = int(parts[its[0]])
-            for index, low in enumerate(lows):
-                for row0 in range(0, packed, height):
-                    bucket.append((entry, low, min(low + step, end), member, row0, min(height, packed - row0), offset + index, fresh))
-            parts[its] += len(lows)
-
-        def listed(bucket) -> np.ndarray:
-            items = np.asarray(bucket, dtype=np.int32).reshape(-1, kernels.SHARED_ITEM)
-            return np.ascontiguousarray(items[np.argsort(items[:, 1] - items[:, 2], kind="stable")])      # the longest first
+        def listed(kind: np.ndarray) -> np.ndarray:
+            chosen = np.flatnonzero(kind)
+            pieces = ranges[chosen] * high[chosen]
+            index = np.repeat(chosen, pieces)
+            place = np.arange(int(pieces.sum())) - np.repeat(np.cumsum(pieces) - pieces, pieces)
+            nth, tile = place // high[index], place % high[index]
+            begin, row0 = work[index, 1] + nth * step[index], tile * height[index]
+            items = np.stack([work[index, 0], begin, np.minimum(begin + step[index], work[index, 2]), work[index, 3], row0,
+                              np.minimum(height[index], work[index, 4] - row0), work[index, 6] + nth, work[index, 5]], 1)
+            return np.ascontiguousarray(items[np.argsort(items[:, 1] - items[:, 2], kind="stable")].astype(np.int32))      # the longest first
 
         part_first = np.concatenate(([0], np.cumsum(parts)))
-        return {"tile_items": listed(tiles), "row_items": listed(rows), "members": np.concatenate(members).astype(np.int32),
+        return {"tile_items": listed(~low), "row_items": listed(low), "members": everyone.astype(np.int32),
                 "part_first": part_first.astype(np.int32), "parts": int(part_first[-1]), "tokens": tokens, "entries": count,
-                "tile_rows": int(tile_rows), "most_rows": int(most), "heads": (self.group, self.num_kv_heads, self.head_dim),
-                "dtype": self.tag}
+                "tile_rows": int(tile_rows), "most_rows": int(np.minimum(work[low, 4], kernels.DECODE_TILE_ROWS).max()) if low.any() else 0,
+                "heads": (self.group, self.num_kv_heads, self.head_dim), "dtype": self.tag}
+
+    def saved_bytes(self, shape: StepShape) -> int:
+        """Bytes of keys and values that the members of the step's groups would read again if each read its own."""
+        groups, shared = np.asarray(shape.prefix_group, dtype=np.int64), np.asarray(shape.prefix_tokens, dtype=np.int64)
+        _, first, count = np.unique(groups, return_index=True, return_counts=True)
+        again = int(((count - 1) * shared[first] * (groups[first] >= 0)).sum())
+        return again * 2 * self.num_kv_heads * self.head_dim * (4 if self.wide else 2)
+
+    def step_plan(self, shape: StepShape) -> dict | None:
+        """The plan of a decode-only step where sharing is worth its launches, else ``None``.  The lists are filled up with empty
+        items and the number of parts is rounded up, to powers of two: what a captured step has baked in then changes at few
+        context lengths."""
+        if not shape.decode_only or shape.prefix_group is None or self.saved_bytes(shape) < (WORTH_SHARING_F32 if self.wide else WORTH_SHARING):
+            return None
+        plan = self.plan(shape)
+        up = lambda n: 0 if n == 0 else 1 << (int(n) - 1).bit_length()
+        for name in ("tile_items", "row_items"):
+            items = plan[name]
+            padded = np.zeros((up(len(items)), kernels.SHARED_ITEM), dtype=np.int32)
+            padded[: len(items)] = items
+            plan[name] = padded
+        if 8 * (len(plan["tile_items"]) + len(plan["row_items"])) > self.capacity(len(shape.lengths), len(shape.lengths)) - 3 * len(shape.lengths) - 64:
+            return None
+        return {**plan, "parts": up(plan["parts"]), "shared": True}
+
+    def capacity(self, max_tokens: int, max_entries: int) -> int:
+        return 8 * (2048 + 8 * max_entries) + 3 * max_entries + 64
+
+
+# Bytes of keys and values, read again by every member but one, from which on a decode step reads shared prefixes once.  Measured
+# with 8 key heads of 128 and groups of 4 in bfloat16, us in a captured step, ordinary against shared, at requests x shared positions:
+# 8 x 1,024 (29 MB) 10.9 and 11.6, 4 x 4,096 (50 MB) 14.1 and 13.5, 32 x 512 (65 MB) 12.3 and 13.6, 2 x 16,384 (67 MB) 23.4 and
+# 25.9, 8 x 4,096 (117 MB) 20.2 and 15.8, 16 x 2,048 (126 MB) 17.8 and 13.2, 64 x 1,024 (264 MB) 36 and 23, 8 x 16,384 (470 MB) 62 and 25.
+WORTH_SHARING = 96 << 20
+WORTH_SHARING_F32 = 8 << 20
+
+
+class SharedSteps(StepPlanner):
+    """A planner of shared prefixes alone, for the float32 path, whose other steps need no lists."""
+
+    def __init__(self, items: SharedItems) -> None:
+        self.items = items
+        self.key = ("shared_steps", *items.key)
+
+    def capacity(self, max_tokens: int, max_entries: int) -> int:
+        return self.items.capacity(max_tokens, max_entries)
+
+    def plan(self, shape: StepShape) -> dict:
+        return self.items.step_plan(shape) or {}
 
 
 @MIXERS.register("gqa_attention")
@@ -465,8 +519,13 @@ class GQAAttention(Mixer):
         if device.type == "cuda" and dtype == torch.bfloat16:
             clusters = kernels.attention_decode_clusters(self.d, device) or None
         plain_scores = not self.softcap
+        # every position before its own is seen, by plain scores, and keys and values lie side by side: prefixes may be shared
+        shared = None
+        if plain_scores and not self.window and not self.chunk and not self.keys_are_values and self.scale > 0:
+            shared = SharedItems(self.hq // self.hkv, self.hkv, self.d, sms, dtype)
         self._items = AttentionItems(self.hq // self.hkv, self.hkv, self.d, sms, clusters if plain_scores else None,
-                                     decode_tensor_core=plain_scores, chunk=self.chunk)
+                                     decode_tensor_core=plain_scores, chunk=self.chunk, shared=shared)
+        self._shared_steps = SharedSteps(shared) if shared is not None and dtype == torch.float32 else None
         self.position = POSITION_ENCODINGS.build(position, dtype=dtype, device=device)
         self.rotary_dim = int(position.params.get("rotary_dim", getattr(self.position, "rotary_dim", self.d)))
 
@@ -519,7 +578,7 @@ class GQAAttention(Mixer):
 
     def step_planner(self) -> StepPlanner | None:
         if self.dtype != torch.bfloat16:
-            return None      # the float32 path runs the one-warp-per-row kernel: no work list
+            return self._shared_steps      # the float32 path runs the one-warp-per-row kernel: no work list but for shared prefixes
         return self._items
 
     # -- weights --------------------------------------------------------------- #
@@ -736,6 +795,19 @@ class GQAAttention(Mixer):
         )
 
     def attend(self, q, pages, out, batch, group, gate=None) -> None:
+        planner = self.step_planner()
+        plan = None if planner is None else batch.extras.get(planner.key)
+        if plan and plan.get("shared"):
+            rows = plan["parts"] * self.hq
+            kernels.attention_shared(
+                q, pages, out, plan=plan,
+                part_out=batch.workspace.get("attn_part_out", rows, self.d, torch.float32, min_rows=rows),
+                part_lse=batch.workspace.get("attn_part_lse", rows, 1, torch.float32, min_rows=rows),
+                positions=batch.positions, cu_seqlens=batch.cu_seqlens, entry_start=batch.entry_start, entry_slot=batch.entry_slot,
+                block_table=group.block_table, num_heads=self.hq, num_kv_heads=self.hkv, head_dim=self.d, scale=self.scale,
+                fault=batch.fault, sink=self.sink, gate=gate, slopes=self.slopes,
+            )
+            return
         if q.dtype == torch.bfloat16:
             plan = batch.extras[self._items.key]
             splits = plan["splits"]

@@ -8,7 +8,9 @@ tokens do not depend on what else is in the batch.  ``stop_on_repeat`` ends a re
 generated text loops (finish reason ``"repeat"``); the test is on decoded text, so it acts only
 when the model folder has a tokenizer, and requests of token ids alone are never ended by it.
 ``logprobs`` and ``prompt_logprobs`` (reporting, not sampling) are accepted only as ``None``;
-any other value is refused at construction rather than ignored.
+any other value is refused at construction rather than ignored.  Three more additions: ``top_k`` keeps the k largest
+logits before ``top_p`` is taken of what they leave (0 = all), ``min_p`` keeps what has at least that share of the largest
+probability (0 = everything), and ``n`` asks for several completions of one prompt, which is computed once for all of them.
 """
 
 from __future__ import annotations
@@ -26,6 +28,9 @@ class SamplingParams:
     logprobs: int | None = None
     prompt_logprobs: int | None = None
     seed: int | None = None
+    top_k: int = 0
+    min_p: float = 0.0
+    n: int = 1
 
     def __post_init__(self) -> None:
         if self.temperature < 0:
@@ -38,6 +43,12 @@ class SamplingParams:
             raise ValueError(f"repetition_penalty must be > 0, got {self.repetition_penalty}")
         if self.logprobs is not None or self.prompt_logprobs is not None:
             raise ValueError("logprobs and prompt_logprobs are not reported by this engine; leave them None")
+        if self.top_k < 0 or self.top_k != int(self.top_k):
+            raise ValueError(f"top_k must be a whole number >= 0 (0 = all), got {self.top_k}")
+        if not 0.0 <= self.min_p <= 1.0:
+            raise ValueError(f"min_p must be in [0, 1], got {self.min_p}")
+        if self.n < 1 or self.n != int(self.n):
+            raise ValueError(f"n must be a whole number >= 1, got {self.n}")
         if self.seed is not None and not 0 <= self.seed < 2**63:
             raise ValueError(f"seed must be in [0, 2**63), got {self.seed}")
 

@@ -1,7 +1,7 @@
 """Turns a step's logits rows into one token per row with the CUDA sampling kernel.
 
 One launch handles a batch whose rows disagree about temperature, top-p and repetition
-penalty, as the reference's batched sampler does with per-row tensors
+penalty (a second one the rows with top-k or min-p), as the reference's batched sampler does with per-row tensors
 (``rapid_llm/engine/sampler.py:448-520,689-696``).  A wholly greedy batch without penalties
 passes no parameter arrays at all; otherwise every per-row parameter of the step (temperatures,
 top-p, penalties, seeds, draw counters, the tokens a penalty looks at) is laid into ONE pinned buffer
@@ -59,7 +59,7 @@ class Sampler:
             kernels.sample(logits, out)
             return
         # one buffer of 32-bit words: temperature, top-p, penalty, counters (rows each), seeds (two words a row,
-        # on an 8-byte boundary), then the offsets and the tokens the penalties look at
+        # on an 8-byte boundary), then the offsets and the tokens the penalties look at, then top-k and min-p if a row has one
         offsets, flat = [0], []
         if use_penalty:
             for p, tokens in zip(params, generated):
@@ -69,7 +69,10 @@ class Sampler:
         at_seeds = (4 * rows + 1) // 2 * 2
         at_offsets = at_seeds + 2 * rows
         at_seen = at_offsets + rows + 1
-        words = at_seen + max(len(flat), 1)
+        at_filters = at_seen + max(len(flat), 1)
+        filtered = [(p.top_k > 0 or p.min_p > 0.0) and not p.is_greedy for p in params]
+        filters = any(filtered)
+        words = at_filters + (2 * rows if filters else 0)
         host = self._staging(words)
         as_float = host.view(np.float32)
         as_float[0:rows] = [p.temperature for p in params]
@@ -80,15 +83,24 @@ class Sampler:
         if use_penalty:
             host[at_offsets:at_seen] = offsets
             host[at_seen : at_seen + len(flat)] = flat
+        if filters:
+            # (-1: the row is chosen by the call without these cuts, as in a batch where no row has them)
+            host[at_filters : at_filters + rows] = [min(p.top_k, 2**31 - 1) if cut else -1 for p, cut in zip(params, filtered)]
+            as_float[at_filters + rows : words] = [p.min_p for p in params]
         device = self._upload(words)
         floats = device[: 3 * rows].view(torch.float32)
-        kernels.sample(
-            logits, out, temperature=floats[:rows], top_p=floats[rows : 2 * rows],
+        arguments = dict(
+            temperature=floats[:rows], top_p=floats[rows : 2 * rows],
             penalty=floats[2 * rows : 3 * rows] if use_penalty else None,
             seeds=device[at_seeds:at_offsets].view(torch.int64), counters=device[3 * rows : 4 * rows],
             seen_tokens=device[at_seen : at_seen + max(len(flat), 1)] if use_penalty else None,
             seen_offsets=device[at_offsets:at_seen] if use_penalty else None,
         )
+        if not all(filtered):
+            kernels.sample(logits, out, **arguments)
+        if filters:
+            kernels.sample(logits, out, top_k=device[at_filters : at_filters + rows],
+                           min_p=device[at_filters + rows : words].view(torch.float32), **arguments)
 
     def _staging(self, words: int) -> np.ndarray:
         """The next pinned buffer of the rotation as int32 words, at least ``words`` long and no longer in use."""
