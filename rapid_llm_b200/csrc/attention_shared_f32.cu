@@ -52,6 +52,7 @@ attention_shared_f32_kernel(const SharedF32Args args) {
   float* row_max = p_tile + kSfKeys * (kSfRows + kSfPad);
   float* row_sum = row_max + kSfRows;
   float* row_scale = row_sum + kSfRows;
+  __shared__ long long places[2][kSfKeys];               // where a block's key rows start (-1: beyond the end), alternating
   __shared__ int row_token[kSfRows], row_pos[kSfRows];
   __shared__ float row_slope[kSfRows];
   constexpr int p_stride = kSfRows + kSfPad;
@@ -78,6 +79,22 @@ attention_shared_f32_kernel(const SharedF32Args args) {
     row_max[r] = -INFINITY;
     row_sum[r] = 0.0f;
   }
+  // a block's page ids are looked up once, by a thread a key, a block ahead of its copies
+  const size_t head_elements = static_cast<size_t>(args.page_size) * d;
+  auto find = [&](int block) {
+    if (tid >= kSfKeys) return;
+    const int j = first + block * kSfKeys + tid;
+    long long place = -1;
+    if (j < end) {
+      const int at = j / args.page_size, page = table[at];
+      if (page < 0 || page >= args.num_pages)
+        atomicOr(args.fault, kFaultPageId);
+      else
+        place = static_cast<long long>((static_cast<size_t>(page) * 2 * args.hkv + kv_head) * head_elements + static_cast<size_t>(j - at * args.page_size) * d);
+    }
+    places[block & 1][tid] = place;
+  };
+  if (n_blocks > 0) find(0);
   __syncthreads();
   const int chunks = d / 4;
   for (int i = tid; i < kSfRows * chunks; i += kSfThreads) {
@@ -89,24 +106,13 @@ attention_shared_f32_kernel(const SharedF32Args args) {
     }
     *reinterpret_cast<float4*>(q_tile + r * stride + c) = v;
   }
-  const size_t head_elements = static_cast<size_t>(args.page_size) * d;
+  const size_t v_plane = static_cast<size_t>(args.hkv) * head_elements;
   auto load = [&](float* tile, int block, int plane) {
-    const int kb = first + block * kSfKeys;
+    const long long* place = places[block & 1];
     for (int i = tid; i < kSfKeys * chunks; i += kSfThreads) {
-      const int r = i / chunks, c = (i - r * chunks) * 4, j = kb + r;
-      bool valid = j < end;
-      const float* src = args.cache;
-      if (valid) {
-        const int at = j / args.page_size, page = table[at];
-        if (page < 0 || page >= args.num_pages) {
-          atomicOr(args.fault, kFaultPageId);
-          valid = false;
-        } else {
-          src += ((static_cast<size_t>(page) * 2 + plane) * args.hkv + kv_head) * head_elements +
-                 static_cast<size_t>(j - at * args.page_size) * d + c;
-        }
-      }
-      sf_copy16(tile + r * stride + c, src, valid);
+      const int r = i / chunks, c = (i - r * chunks) * 4;
+      const long long at = place[r];
+      sf_copy16(tile + r * stride + c, args.cache + (at < 0 ? 0 : at + static_cast<long long>(plane * v_plane) + c), at >= 0);
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
@@ -127,6 +133,7 @@ attention_shared_f32_kernel(const SharedF32Args args) {
   }
   for (int b = 0; b < n_blocks; ++b) {
     const int kb = first + b * kSfKeys;
+    if (b + 1 < n_blocks) find(b + 1);
     asm volatile("cp.async.wait_group 1;\n" ::: "memory");      // the keys are there, the values may still fly
     __syncthreads();
     {

@@ -6,6 +6,8 @@
 // that no page is written twice and none both read and written, so the order of the CTAs does not matter.  Rows of any size are
 // taken (per-request states are copied by the same kernel): the unit of a copy is the largest of 16, 8, 4, 2 and 1
 // bytes that a page is a multiple of and its address aligned to.
+#include <stdlib.h>
+
 #include "common.cuh"
 
 namespace rl {
@@ -18,7 +20,7 @@ struct PagePairs {
   int2 of[kPairs];
 };
 // A list travels in a block of constants of the launch: a short one keeps the launch short, a long one keeps launches few.
-constexpr int kFewPairs = 120, kManyPairs = 3900;
+constexpr int kFewPairs = 60, kSomePairs = 500, kManyPairs = 3900;
 
 template <typename U, int kPairs>
 __global__ void __launch_bounds__(kCopyThreads)
@@ -66,6 +68,8 @@ static int copy_as(void* pages, const int* pairs, int count, int layers, long lo
     const int left = count - at, take = left <= kFewPairs ? left : left < kManyPairs ? left : kManyPairs;
     const int status = take <= kFewPairs
                            ? launch_copy<U, kFewPairs>(pages, pairs + 2 * at, take, layers, layer_bytes, page_bytes, pdl, stream)
+                       : take <= kSomePairs
+                           ? launch_copy<U, kSomePairs>(pages, pairs + 2 * at, take, layers, layer_bytes, page_bytes, pdl, stream)
                            : launch_copy<U, kManyPairs>(pages, pairs + 2 * at, take, layers, layer_bytes, page_bytes, pdl, stream);
     if (status != 0) return status;
     at += take;
@@ -80,8 +84,31 @@ extern "C" {
 // Launches a list of `count` pairs takes.
 int rl_copy_pages_launches(int count) { return (count + rl::kManyPairs - 1) / rl::kManyPairs; }
 
+// What the pairs of a list break: 0 nothing, -1 a page outside the `known`, -2 a page that is written twice, or read and written,
+// -3 no memory for the check.
+int rl_copy_pages_check(const int* pairs, int count, long long known) {
+  for (int i = 0; i < 2 * count; ++i)
+    if (pairs[i] < 0 || pairs[i] >= known) return -1;
+  if (count <= 32) {
+    for (int i = 0; i < count; ++i)
+      for (int j = 0; j < count; ++j)
+        if ((i != j && pairs[2 * i + 1] == pairs[2 * j + 1]) || pairs[2 * i + 1] == pairs[2 * j]) return -2;
+    return 0;
+  }
+  unsigned char* used = static_cast<unsigned char*>(calloc(static_cast<size_t>(known), 1));
+  if (used == nullptr) return -3;
+  int status = 0;
+  for (int i = 0; i < count; ++i) used[pairs[2 * i]] = 1;
+  for (int i = 0; i < count && status == 0; ++i) {
+    if (used[pairs[2 * i + 1]]) status = -2;
+    used[pairs[2 * i + 1]] = 1;
+  }
+  free(used);
+  return status;
+}
+
 // pages: `layers` blocks of layer_bytes, page p of each at p * page_bytes; pairs: [count, 2] int32 in host memory, read
-// before the call returns.  The caller has checked the ids against the number of pages.
+// before the call returns.  The caller has had the pairs checked.
 int rl_copy_pages(void* pages, const int* pairs, int count, int layers, long long layer_bytes, long long page_bytes, int pdl,
                   cudaStream_t stream) {
   if (count == 0 || layers == 0 || page_bytes == 0) return 0;

@@ -28,7 +28,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 256;
 constexpr int kList = 256;
 constexpr int kMaxRanks = 8;
-constexpr int kMaxSlice = 48 * 1024;          // floats of one CTA's slice (192 KB)
+constexpr int kMaxSlice = 48 * 1024;          // numbers of one CTA's slice (192 KB as floats)
 constexpr int kCodeBits = 23;
 constexpr double kUnit = 8796093022208.0;     // 2^43: a weight of one
 constexpr float kNegligible = 31.0f;          // (m - x) / T beyond which a weight rounds to zero (44 ln 2 = 30.5)
@@ -137,10 +137,10 @@ struct Shared {
   unsigned above_n, inside_n, whole_n;
 };
 
-template <typename T>
+template <typename Store>
 struct Row {
   Shared& s;
-  float* values;
+  Store* values;
   unsigned ranks, rank;
   int begin, count, chunk;      // this CTA's slice; tokens of a thread
   int turn = 0;                 // of the exchange buffers
@@ -148,7 +148,7 @@ struct Row {
   float top, floor_value, code_scale;
   double per, wide_top;
 
-  __device__ Row(Shared& shared, float* v) : s(shared), values(v) {}
+  __device__ Row(Shared& shared, Store* v) : s(shared), values(v) {}
 
   // ---- reductions: over the CTA, then over the cluster; every thread gets the results -------------------------
   struct Sum { __device__ static u64 of(u64 a, u64 b) { return a + b; } };
@@ -218,7 +218,7 @@ struct Row {
   __device__ __forceinline__ void sweep(Fn&& fn) {
     const int first = min(count, static_cast<int>(threadIdx.x) * chunk), last = min(count, first + chunk);
 #pragma unroll 4
-    for (int i = first; i < last; ++i) fn(i, values[i]);
+    for (int i = first; i < last; ++i) fn(i, to_float(values[i]));
   }
   // 23-bit code of the distance to the maximum, or more than that for what lies outside
   __device__ __forceinline__ unsigned code(float x) const {
@@ -411,7 +411,7 @@ struct Row {
   }
 };
 
-constexpr int kRoomySlice = 24 * 1024;        // floats of a slice of which two fit a multiprocessor
+constexpr int kRoomyBytes = 96 * 1024;        // of a slice of which two fit a multiprocessor
 
 static int sm_count() {
   int device = 0, sms = 0;
@@ -419,14 +419,17 @@ static int sm_count() {
   return sms;
 }
 
-template <typename T>
+// Store: what a slice is kept as: floats, or 16-bit logits as they are (half the shared memory, so that fewer CTAs hold a row).
+template <typename T, typename Store>
 __global__ void __launch_bounds__(kThreads, 2)
 sample_filtered_kernel(const Args args, unsigned ranks) {
-  extern __shared__ __align__(16) float slice_values[];
+  using R = Row<Store>;
+  extern __shared__ __align__(16) unsigned char slice_bytes[];
+  Store* slice_values = reinterpret_cast<Store*>(slice_bytes);
   __shared__ Shared s;
   pdl_trigger();
   const int row_index = blockIdx.y;
-  Row<T> row(s, slice_values);
+  R row(s, slice_values);
   row.ranks = ranks;
   row.rank = blockIdx.x;
   row.begin = min(args.vocab, static_cast<int>(row.rank) * args.slice);
@@ -472,13 +475,20 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
         v[j] = clean(to_float(values[j]));
         if (!penalised) seen(c + j, v[j]);
       }
-      *reinterpret_cast<float4*>(slice_values + c) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(slice_values + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      if constexpr (sizeof(Store) == 4) {
+        *reinterpret_cast<float4*>(slice_values + c) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(slice_values + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        __nv_bfloat162 two[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) two[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);      // exact: they were bfloat16
+        *reinterpret_cast<uint4*>(slice_values + c) = *reinterpret_cast<const uint4*>(two);
+      }
     }
   }
   for (int i = vector_count + threadIdx.x; i < row.count; i += kThreads) {
     const float v = clean(to_float(x[i]));
-    slice_values[i] = v;
+    slice_values[i] = from_float<Store>(v);
     if (!penalised) seen(i, v);
   }
   __syncthreads();
@@ -490,14 +500,14 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       bool first = true;
       for (int j = seen_begin; j < i && first; ++j) first = args.seen_tokens[j] != id + row.begin;
       if (first) {
-        const float v = slice_values[id];
-        slice_values[id] = clean(v < 0.0f ? v * pen : v / pen);
+        const float v = to_float(slice_values[id]);
+        slice_values[id] = from_float<Store>(clean(v < 0.0f ? v * pen : v / pen));
       }
     }
     __syncthreads();
     row.sweep(seen);
   }
-  row.template cluster_all<typename Row<T>::Most>(ends);
+  row.template cluster_all<typename R::Most>(ends);
   float top = unordered(static_cast<unsigned>(ends[0] >> 32));
   if (ends[0] == 0ull || !(top > -INFINITY) || !(temp > 0.0f)) {
     // nothing to choose from, or the first maximum; nobody leaves while its shared memory may be read
@@ -507,7 +517,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   }
   float bottom = unordered(~static_cast<unsigned>(ends[1]));
   if (top == INFINITY) {                             // entries of +infinity share everything
-    row.sweep([&](int i, float v) { slice_values[i] = v == INFINITY ? 0.0f : -INFINITY; });
+    row.sweep([&](int i, float v) { slice_values[i] = from_float<Store>(v == INFINITY ? 0.0f : -INFINITY); });
     top = bottom = 0.0f;
     __syncthreads();
   }
@@ -550,7 +560,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   int cut_i = 0x7fffffff;
   auto everything = [](int, float) { return true; };
   if (by_rank) {
-    typename Row<T>::Interval at = {0u, kLast, 0u, 0u, 0.0};
+    typename R::Interval at = {0u, kLast, 0u, 0u, 0.0};
     double unused = 0.0;
     bool fewer = false;
     for (bool first = true;; first = false) {
@@ -651,7 +661,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   u64 weighed = 0;                                   // of this thread's chunk: the mass of codes below `weighed_to`, all of which stays
   unsigned weighed_to = 0;
   if (by_mass) {
-    typename Row<T>::Interval at = {0u, kLast, 0u, 0u, 0.0};
+    typename R::Interval at = {0u, kLast, 0u, 0u, 0.0};
     double whole = -1.0;
     for (int level = 0; level < 3; ++level) {
       row.template narrow<true>(at, 0u, fmax(static_cast<double>(p), 0.0), whole, in_k);
@@ -668,7 +678,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
         ends_of[0] = ordered(s.all_x[threadIdx.x]);
         ends_of[1] = ~ordered(s.all_x[threadIdx.x]);
       }
-      row.template block_all<typename Row<T>::Most>(ends_of);
+      row.template block_all<typename R::Most>(ends_of);
       high = unordered(static_cast<unsigned>(ends_of[0]));
       low = unordered(~static_cast<unsigned>(ends_of[1]));
     }
@@ -687,7 +697,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
         else if (q <= kLast) behind += 1;
       });
       u64 sums[4] = {z, above, inside, behind};
-      row.template cluster_all<typename Row<T>::Sum>(sums);
+      row.template cluster_all<typename R::Sum>(sums);
       weighed = above;
       weighed_to = at.low;
       z = sums[0];
@@ -717,7 +727,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
           near_n += 1;
         });
         u64 near_sums[2] = {near_mass, near_n};
-        row.template cluster_all<typename Row<T>::Sum>(near_sums);
+        row.template cluster_all<typename R::Sum>(near_sums);
         near_mass = near_sums[0];
         near_n = near_sums[1];
         if (static_cast<double>(above + near_mass) <= budget && near_n < at.inside_n) {
@@ -739,7 +749,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
           if (static_cast<double>(mass) <= budget) best = ~ordered(my_x);
         }
         u64 one[1] = {best};
-        row.template block_all<typename Row<T>::Most>(one);
+        row.template block_all<typename R::Most>(one);
         cut_p = unordered(~static_cast<unsigned>(one[0]));
         __syncthreads();
       } else {
@@ -767,7 +777,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
         best = ~static_cast<unsigned>(row.begin + i);
     });
     u64 one[1] = {best};
-    row.template cluster_all<typename Row<T>::Most>(one);
+    row.template cluster_all<typename R::Most>(one);
     if (row.rank == 0 && threadIdx.x == 0) args.out[row_index] = static_cast<int>(~static_cast<unsigned>(one[0]));
     if (ranks > 1) cluster_barrier();
     return;
@@ -823,7 +833,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
     const int first = (warp * 32 + source) * row.chunk, last = min(row.count, first + row.chunk);
     for (int i0 = first; i0 < last; i0 += 32) {
       const int i = i0 + lane;
-      const u64 w = i < last ? kept_weight(i, slice_values[i]) : 0ull;
+      const u64 w = i < last ? kept_weight(i, to_float(slice_values[i])) : 0ull;
       u64 sum = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -857,21 +867,23 @@ int rl_sample_filtered(int dtype, const void* logits, int rows, int vocab, long 
   if (rows < 0 || rows > 65535 || vocab <= 0 || vocab > rl_sample_filtered_max_vocab() ||
       (temperature != nullptr && uniforms == nullptr && (seeds == nullptr || counters == nullptr)))
     return static_cast<int>(cudaErrorInvalidValue);
-  // CTAs a row: as many as run at one time (two a multiprocessor), since a row's steps wait for one another more than they
-  // compute, and enough that a slice leaves room for two
-  const int slots = 2 * rl::filters::sm_count();
+  // A penalty makes a logit wider than 16 bits.
+  const bool halves = dtype == rl::kBF16 && (penalty == nullptr || seen_tokens == nullptr);
+  const int size = halves ? 2 : 4, slots = 2 * rl::filters::sm_count();
+  // CTAs a row: as many as run at one time (two a multiprocessor), since a row's steps wait for one another more than they compute, as
+  // long as two slices fit.  With 8 and with fewer: 256 rows of 32,003 107 and 31 us (1), 64 rows of 151,936 with top-k 47 and
+  // 36 (4); that disagree about everything 78 and 82; one row 19 and 27.
   int ranks = rl::filters::kMaxRanks;
-  while (ranks > 1 && rows * ranks > slots && (vocab + ranks / 2 - 1) / (ranks / 2) <= rl::filters::kRoomySlice) ranks /= 2;
+  while (ranks > 1 && rows * ranks > slots && ((vocab + ranks / 2 - 1) / (ranks / 2) + 8) * size <= rl::filters::kRoomyBytes) ranks /= 2;
   rl::filters::Args a = {};
   a.logits = logits; a.row_stride = row_stride; a.vocab = vocab;
   a.slice = ((vocab + ranks - 1) / ranks + 7) & ~7;
   a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.penalty = penalty; a.uniforms = uniforms;
   a.seeds = seeds; a.counters = counters; a.seen_tokens = seen_tokens; a.seen_offsets = seen_offsets; a.out = out;
-  const size_t bytes = static_cast<size_t>(a.slice) * sizeof(float);
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(ranks, rows);
   config.blockDim = dim3(rl::filters::kThreads);
-  config.dynamicSmemBytes = bytes;
+  config.dynamicSmemBytes = static_cast<size_t>(a.slice) * size;
   config.stream = stream;
   cudaLaunchAttribute attributes[2];
   attributes[0].id = cudaLaunchAttributeClusterDimension;
@@ -882,14 +894,16 @@ int rl_sample_filtered(int dtype, const void* logits, int rows, int vocab, long 
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = ranks > 1 ? attributes : attributes + 1;      // a row in one CTA needs no cluster
   config.numAttrs = (ranks > 1 ? 1 : 0) + (pdl ? 1 : 0);
-  RL_DISPATCH_DTYPE(dtype, {
-    static std::atomic<unsigned long long> configured;
-    auto kernel = rl::filters::sample_filtered_kernel<scalar_t>;
-    const cudaError_t e = rl::allow_shared(kernel, rl::filters::kMaxSlice * static_cast<int>(sizeof(float)), configured);
+  static std::atomic<unsigned long long> configured[3];
+  auto launch = [&](auto kernel, int which) {
+    const cudaError_t e = rl::allow_shared(kernel, rl::filters::kMaxSlice * size, configured[which]);
     if (e != cudaSuccess) return static_cast<int>(e);
     return static_cast<int>(cudaLaunchKernelEx(&config, kernel, a, static_cast<unsigned>(ranks)));
-  });
-  return 0;
+  };
+  if (dtype == rl::kF32) return launch(rl::filters::sample_filtered_kernel<float, float>, 0);
+  if (dtype != rl::kBF16) return static_cast<int>(cudaErrorInvalidValue);
+  return halves ? launch(rl::filters::sample_filtered_kernel<__nv_bfloat16, __nv_bfloat16>, 1)
+                : launch(rl::filters::sample_filtered_kernel<__nv_bfloat16, float>, 2);
 }
 
 }  // extern "C"

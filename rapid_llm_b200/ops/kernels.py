@@ -74,6 +74,17 @@ def _need_cuda(*tensors: torch.Tensor | None) -> None:
             )
 
 
+def _need_here(*tensors: torch.Tensor | None) -> None:
+    """Every tensor on the current device, whose stream the launch goes to."""
+    here = None
+    for tensor in tensors:
+        if tensor is not None and tensor.get_device() != here:
+            _need_cuda(tensor)
+            here = torch.cuda.current_device()
+            if tensor.get_device() != here:
+                raise KernelError(f"kernel arguments must live on the current device (cuda:{here}), got a tensor on {tensor.device}")
+
+
 def _contig(name: str, tensor: torch.Tensor | None) -> None:
     if tensor is not None and not tensor.is_contiguous():
         raise KernelError(f"{name} must be contiguous")
@@ -151,6 +162,7 @@ def core() -> ctypes.CDLL:
         ]
         lib.rl_copy_pages.argtypes = [c_void_p, c_void_p, c_int, c_int, c_longlong, c_longlong, c_int, c_void_p]
         lib.rl_copy_pages_launches.argtypes = [c_int]
+        lib.rl_copy_pages_check.argtypes = [c_void_p, c_int, c_longlong]
         lib.rl_embedding_sum.argtypes = [
             c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
             c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_int, c_float,
@@ -170,7 +182,7 @@ def core() -> ctypes.CDLL:
         for name in (
             "rl_sample_filtered", "rl_sample_filtered_max_vocab", "rl_embedding", "rl_embedding_sum", "rl_scatter_rows", "rl_add_rmsnorm", "rl_silu_mul", "rl_to_float", "rl_clamped_glu",
             "rl_rope_unit_write", "rl_layernorm", "rl_row_norm_rope_write", "rl_sigmoid_gate", "rl_relu_squared",
-            "rl_qk_norm_rope_write", "rl_attention_generic", "rl_attention_shared_f32", "rl_copy_pages", "rl_copy_pages_launches", "rl_gemm_f32", "rl_sample",
+            "rl_qk_norm_rope_write", "rl_attention_generic", "rl_attention_shared_f32", "rl_copy_pages", "rl_copy_pages_launches", "rl_copy_pages_check", "rl_gemm_f32", "rl_sample",
         ):
             getattr(lib, name).restype = c_int
         if lib.rl_attention_shared_f32_rows() != SHARED_F32_ROWS:
@@ -252,7 +264,7 @@ def copy_pages(pages: torch.Tensor, pairs) -> torch.Tensor:
 
     ``pairs`` is on the host (a sequence of pairs or an integer array ``[n, 2]``); it is read before the call returns.
     No target may be named twice or be a source too: the copies run side by side, in no order."""
-    _need_cuda(pages)
+    _need_here(pages)
     _contig("pages", pages)
     if pages.dim() < 2:
         raise KernelError("copy_pages: pages must be [layers, pages, *page]")
@@ -261,18 +273,18 @@ def copy_pages(pages: torch.Tensor, pairs) -> torch.Tensor:
         return pages
     if pairs.dtype.kind not in "iu" or pairs.ndim != 2 or pairs.shape[1] != 2:
         raise KernelError("copy_pages: pairs must be integers [n, 2]")
-    sources, targets = pairs[:, 0].tolist(), pairs[:, 1].tolist()
-    known = pages.shape[1]
-    if min(sources) < 0 or min(targets) < 0 or max(sources) >= known or max(targets) >= known:
-        raise KernelError(f"copy_pages: a pair names a page outside the {known} there are")
-    written = set(targets)
-    if len(written) != len(targets) or not written.isdisjoint(sources):
-        raise KernelError("copy_pages: a page is written twice, or both read and written")
     listed = np.ascontiguousarray(pairs, dtype=np.int32)
+    if pairs.dtype.itemsize > 4 and (listed != pairs).any():
+        raise KernelError("copy_pages: a page's number does not fit 32 bits")
+    count, known, lib = listed.shape[0], pages.shape[1], core()
+    broken = lib.rl_copy_pages_check(listed.ctypes.data, count, known)
+    if broken:
+        raise KernelError("copy_pages: " + {-1: f"a pair names a page outside the {known} there are",
+                                            -2: "a page is written twice, or both read and written"}.get(broken, "no host memory"))
     size = pages.element_size()
-    _check(core().rl_copy_pages(_ptr(pages), listed.ctypes.data, len(targets), pages.shape[0], pages.stride(0) * size,
-                                pages.stride(1) * size, int(PDL), _stream()), "copy_pages")
-    LAUNCHES.count += core().rl_copy_pages_launches(len(targets)) - 1
+    _check(lib.rl_copy_pages(_ptr(pages), listed.ctypes.data, count, pages.shape[0], pages.stride(0) * size,
+                             pages.stride(1) * size, int(PDL), _stream()), "copy_pages")
+    LAUNCHES.count += lib.rl_copy_pages_launches(count) - 1
     return pages
 
 
@@ -843,7 +855,7 @@ def attention_shared(
     ``[part_rows, head_dim]`` and ``part_lse`` ``[part_rows]`` (float32) are scratch of ``SharedItems.part_rows(plan)`` rows
     and more; calls that may run at the same time need scratch of their own.  ``sink``, ``gate`` and ``slopes`` as in :func:`attention_mma`, rows of ``out`` and
     ``gate`` too; every key up to a token's own position is seen (no window, no squashed scores, caches of two planes)."""
-    _need_cuda(q, cache, out, part_out, part_lse, positions, cu_seqlens, entry_start, entry_slot, block_table, fault, sink, gate, slopes)
+    _need_here(q, cache, out, part_out, part_lse, positions, cu_seqlens, entry_start, entry_slot, block_table, fault, sink, gate, slopes)
     _per_head(num_heads, sink=sink, slopes=slopes)
     _contig("q", q), _contig("cache", cache)
     for name, tensor in (("positions", positions), ("cu_seqlens", cu_seqlens), ("entry_start", entry_start),
@@ -863,7 +875,7 @@ def attention_shared(
     out_stride, gate_stride = _attention_out(out, gate, tokens, num_heads, head_dim)
     tile_items, row_items = plan["tile_items"], plan["row_items"]
     members, part_first = plan["members"], plan["part_first"]
-    _need_cuda(tile_items, row_items, members, part_first)
+    _need_here(tile_items, row_items, members, part_first)
     for name, tensor in (("tile_items", tile_items), ("row_items", row_items), ("members", members), ("part_first", part_first)):
         _expect(name, tensor, torch.int32), _contig(name, tensor)
     need = plan["parts"] * num_heads
@@ -1282,6 +1294,7 @@ def sample(
 
 
 def _sample_filtered(logits, out, temperature, top_k, top_p, min_p, penalty, uniforms, seeds, counters, seen_tokens, seen_offsets):
+    _need_here(logits, out, temperature, top_k, top_p, min_p, penalty, uniforms, seeds, counters, seen_tokens, seen_offsets)
     rows = logits.shape[0]
     if logits.dim() != 2 or logits.stride(1) != 1 or out.numel() != rows:
         raise KernelError("sample: logits must be [rows, vocab] with contiguous rows and out [rows]")

@@ -262,8 +262,8 @@ class SharedItems(StepPlanner):
         return plan["parts"] * self.group * self.num_kv_heads
 
     # Measured times in microseconds by the rows of a tile: an item's start (page ids, queries, first keys, result), a block of 128
-    # keys, and how many items a multiprocessor runs at one time; the join of the parts: its start, a part, a part of 1,024 rows.
-    COSTS = {256: (7.0, 1.7, 1), 128: (6.0, 0.95, 1), 64: (4.0, 1.2, 2), 32: (5.0, 5.0, 2), 16: (3.0, 0.9, 3)}
+    # keys (64 in the float32 tiles of 32 rows), and how many items a multiprocessor runs at one time; the join of the parts: its start, a part, a part of 1,024 rows.
+    COSTS = {256: (7.0, 1.7, 1), 128: (6.0, 0.95, 1), 64: (4.0, 1.2, 2), 32: (5.0, 4.0, 2), 16: (3.0, 0.9, 3)}
     JOIN = (2.0, 0.05, 0.35)
     STEPS = np.array([1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64, 96, 128, 192, 256, 512, 1024, 4096, 1 << 20])
 
@@ -333,7 +333,7 @@ class SharedItems(StepPlanner):
         else:
             tile_rows = kernels.SHARED_TC_ROWS[int(work[:, 4].max()) > kernels.SHARED_TC_ROWS[0]]
         height = np.where(low, kernels.DECODE_TILE_ROWS, tile_rows)
-        block = kernels.DECODE_TC_KEYS
+        block = kernels.MMA_KEYS if self.wide else kernels.DECODE_TC_KEYS
         blocks, high = -(-(work[:, 2] - work[:, 1]) // block), -(-work[:, 4] // height)
         tile_step, row_step = self._blocks_per_item(np.stack([blocks, high * self.num_kv_heads], 1)[~low],
                                                     np.stack([blocks, high * self.num_kv_heads], 1)[low], tile_rows, tokens)
@@ -398,7 +398,9 @@ class SharedItems(StepPlanner):
 # 8 x 1,024 (29 MB) 10.9 and 11.6, 4 x 4,096 (50 MB) 14.1 and 13.5, 32 x 512 (65 MB) 12.3 and 13.6, 2 x 16,384 (67 MB) 23.4 and
 # 25.9, 8 x 4,096 (117 MB) 20.2 and 15.8, 16 x 2,048 (126 MB) 17.8 and 13.2, 64 x 1,024 (264 MB) 36 and 23, 8 x 16,384 (470 MB) 62 and 25.
 WORTH_SHARING = 96 << 20
-WORTH_SHARING_F32 = 8 << 20
+# ... and in float32, where the other kernel gives every row a warp of its own: 8 heads in groups of 4, 2 x 64 (0.02 MB) 22 and 8 us,
+# 8 x 128 39 and 11, 8 x 2,048 566 and 13.
+WORTH_SHARING_F32 = 0
 
 
 class SharedSteps(StepPlanner):

@@ -79,7 +79,7 @@ def test_a_captured_call_keeps_its_pairs():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("pairs", [[(0, 9)], [(-1, 0)], [(9, 0)], [(0, -2)], [(0, 1), (2, 1)], [(0, 1), (1, 2)], [(3, 3)],
-                                   [(0, 1, 2)], [(0.5, 1.0)], [0, 1]], ids=str)
+                                   [(0, 1, 2)], [(0.5, 1.0)], [0, 1], [(2**32, 1)], [(2**40, 2**33 + 1)]], ids=str)
 def test_refused(pairs):
     pages = torch.randn((2, 9, 32), device=DEV)
     before = pages.clone()
@@ -87,6 +87,19 @@ def test_refused(pairs):
         kernels.copy_pages(pages, pairs)
     assert torch.equal(pages, before)
     assert kernels.copy_pages(pages, []) is pages
+
+
+@pytest.mark.gpu
+def test_long_lists_are_looked_over_too():
+    pages = torch.randn((1, 300, 4), device=DEV)
+    before = pages.clone()
+    good = [(i, 150 + i) for i in range(140)]
+    for wrong in ((3, 160), (160, 299), (299, 5), (0, 300), (-1, 299), (298, 298)):
+        with pytest.raises(kernels.KernelError):
+            kernels.copy_pages(pages, good + [wrong])
+    assert torch.equal(pages, before)
+    kernels.copy_pages(pages, good + [(149, 299), (0, 298)])
+    assert torch.equal(pages[0, 150:290], before[0, :140]) and torch.equal(pages[0, 298], before[0, 0])
 
 
 @pytest.mark.gpu
