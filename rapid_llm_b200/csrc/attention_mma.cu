@@ -970,7 +970,7 @@ int rl_attention_mma(const void* q, const void* cache, void* out, float* part_ou
 // second starts while the first still runs (both read the queries and write parts of their own), the join waits for both.
 int rl_attention_shared(const void* q, const void* cache, void* out, float* part_out, float* part_lse, const int* tile_items,
                         int n_tile_items, int tile_rows, const int* row_items, int n_row_items, int most_rows,
-                        const int* members, const int* positions, const int* part_first, const int* entry_slot,
+                        const int* members, const int* positions, const int* part_first, long long parts, const int* entry_slot,
                         const int* block_table, int tokens, int hq, int hkv, int head_dim, int page_size, int num_pages,
                         int max_pages, int slots, float scale, const float* sink, const float* slopes, int out_stride,
                         const void* gate, int gate_stride, int* fault, int pdl, cudaStream_t stream) {
@@ -980,7 +980,7 @@ int rl_attention_shared(const void* q, const void* cache, void* out, float* part
       (tile_rows != 64 && !attn::decode_tc_supported(page_size)) ||
       static_cast<long long>(num_pages) * 2 * hkv * page_size > 0x7fffffffll || out_stride < hq * head_dim || out_stride % 8 != 0 ||
       (reinterpret_cast<uintptr_t>(out) & 15) || (gate != nullptr && gate_stride < hq) ||
-      static_cast<long long>(tokens) * hq > 0x7fffffffll)
+      static_cast<long long>(tokens) * hq > 0x7fffffffll || parts < 0 || parts * hq > 0x7fffffffll)
     return static_cast<int>(cudaErrorInvalidValue);
   attn::AttentionArgs args = {};
   args.q = static_cast<const attn::bf16*>(q);

@@ -58,7 +58,7 @@ __device__ __forceinline__ void rw_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
 __device__ __forceinline__ uint32_t rw_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 template <int kOctets, bool kSloped>
-__global__ void __launch_bounds__(kRwWarps * 32, kOctets == 1 ? 3 : 2)
+__global__ void __launch_bounds__(kRwWarps * 32, kOctets == 1 ? 4 : 2)
 attention_rows_kernel(const RowsArgs args) {
   constexpr int kSegs = kD / 32, kRounds = kD / 64, kTiles = kD / 16;
   __shared__ int staged_pages[kRwStagedPages];
@@ -84,17 +84,16 @@ attention_rows_kernel(const RowsArgs args) {
   const int* table = args.block_table + static_cast<size_t>(bad ? 0 : slot) * args.max_pages;
   const int begin = first & ~(kRwKeys - 1);
   const int steps = end > first ? (end - begin + kRwKeys - 1) / kRwKeys : 0;
-  const int first_page = begin / args.page_size;
-  const int page_count = steps > 0 ? (end - 1) / args.page_size - first_page + 1 : 0;
-  const bool staged = page_count <= kRwStagedPages;
   auto checked = [&](int page) {
     if (page >= 0 && page < args.num_pages) return page;
     atomicOr(args.fault, kFaultPageId);
     return 0;                                  // the null page: readable
   };
-  if (staged)
-    for (int i = tid; i < page_count; i += kRwWarps * 32) staged_pages[i] = checked(table[first_page + i]);
-  auto page_at = [&](int index) { return staged ? staged_pages[index - first_page] : checked(table[index]); };
+  // With pages of 16 and its multiples a step's keys lie in one page: a lane looks up the page of the warp's step that
+  // has its number, and of every 32nd behind it.  Other pages: all ids of the range are brought to shared memory.
+  const bool in_page = args.page_size % kRwKeys == 0;
+  auto page_of_step = [&](int step) { return step < steps ? table[(begin + step * kRwKeys) / args.page_size] : 0; };
+  int my_page = in_page ? page_of_step(warp + kRwWarps * lane) : 0;
 
   // this lane's rows: operands of row g (of each octet), scores and sums of rows 2 c and 2 c + 1
   int limit[kOctets][2], pos[kOctets][2];
@@ -113,7 +112,15 @@ attention_rows_kernel(const RowsArgs args) {
     const int r = min(o * 8 + g, rows - 1), p = row0 + r;        // rows behind the last repeat it; nothing of theirs is kept
     q_at[o] = (static_cast<size_t>(members[p / group]) * args.hq + kv_head * group + p % group) * kD;
   }
-  __syncthreads();
+  const int first_page = begin / args.page_size;
+  const int page_count = steps > 0 ? (end - 1) / args.page_size - first_page + 1 : 0;
+  const bool staged = !in_page && page_count <= kRwStagedPages;
+  if (!in_page) {
+    if (staged)
+      for (int i = tid; i < page_count; i += kRwWarps * 32) staged_pages[i] = checked(table[first_page + i]);
+    __syncthreads();
+  }
+  auto page_at = [&](int index) { return staged ? staged_pages[index - first_page] : checked(table[index]); };
   if (!args.early) pdl_wait();                 // queries and this step's keys come from the kernels before
 #pragma unroll
   for (int o = 0; o < kOctets; ++o)
@@ -122,7 +129,6 @@ attention_rows_kernel(const RowsArgs args) {
 
   const size_t v_plane = static_cast<size_t>(args.hkv) * args.page_size * kD;
   const bf16* head = args.cache + static_cast<size_t>(kv_head) * args.page_size * kD;
-  const bool in_page = args.page_size % kRwKeys == 0;            // a step's keys lie in one page
   // where key j's row starts; keys outside the range read the nearest one inside, and weigh nothing
   auto row_of = [&](int j) {
     const int at = min(max(j, first), end - 1), index = at / args.page_size;
@@ -143,15 +149,20 @@ attention_rows_kernel(const RowsArgs args) {
       for (int e = 0; e < 4; ++e) out[o][t][e] = 0.0f;
   }
 
-  for (int step = warp; step < steps; step += kRwWarps) {
+  int nth = 0;
+  for (int step = warp; step < steps; step += kRwWarps, ++nth) {
     const int kb = begin + step * kRwKeys;
     uint4 ka[kSegs], kc[kSegs], v[kRounds][4];
     {
       const bf16 *k_near, *k_far, *v_row[4];
       if (in_page) {
-        const int index = kb / args.page_size;
-        const bf16* base = head + static_cast<size_t>(page_at(index)) * 2 * v_plane;
-        const int at = kb - index * args.page_size, low = max(first - kb, 0), high = min(end - kb, kRwKeys) - 1;
+        if (nth == 32) {
+          nth = 0;
+          my_page = page_of_step(step + kRwWarps * lane);
+        }
+        const int page = checked(__shfl_sync(0xffffffffu, my_page, nth));
+        const bf16* base = head + static_cast<size_t>(page) * 2 * v_plane;
+        const int at = kb % args.page_size, low = max(first - kb, 0), high = min(end - kb, kRwKeys) - 1;
         auto inside = [&](int i) { return base + static_cast<size_t>(at + min(max(i, low), high)) * kD; };
         k_near = inside(g);
         k_far = inside(g + 8);

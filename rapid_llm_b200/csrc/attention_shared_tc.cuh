@@ -74,6 +74,7 @@ attention_shared_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
   __shared__ uint32_t tmem_slot;
   __shared__ int aborted_flag;
   __shared__ int staged_pages[kShStagedPages];
+  __shared__ int part_rows[kQTiles * kShTileRows];       // where each row's result goes
   volatile int* aborted = &aborted_flag;
 
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
@@ -283,6 +284,9 @@ attention_shared_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
     const int head = kv_head * group + p % group;
     const int pos = valid ? args.positions[token] : -1;
     const int limit = min(pos, k_end - 1);             // last key the row sees here
+    const int q_row = token * args.hq + head;
+    const int part_row = (args.part_first[token] + part) * args.hq + head;
+    if (kTwoTiles || st == 0) part_rows[tile * kShTileRows + r] = part_row;
     pdl_wait();                                        // queries come from the kernel before
     pdl_trigger();                                     // from here on nothing that follows needs to wait for that one
     if (kTwoTiles || st == 0) {
@@ -291,11 +295,9 @@ attention_shared_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int rr = quarter * 32 + 2 * i + (lane >> 4);
-        const int pp = row0 + tile * kShTileRows + rr;
+        const int from = __shfl_sync(0xffffffffu, q_row, rr & 31);       // (a lane knows its own row)
         fetched[i] = make_uint4(0, 0, 0, 0);
-        if (rr < rows_here)
-          fetched[i] = __ldcg(reinterpret_cast<const uint4*>(
-              args.q + (static_cast<size_t>(members[pp / group]) * args.hq + kv_head * group + pp % group) * kShD + (lane & 15) * 8));
+        if (rr < rows_here) fetched[i] = __ldcg(reinterpret_cast<const uint4*>(args.q + static_cast<size_t>(from) * kShD + (lane & 15) * 8));
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -468,18 +470,15 @@ attention_shared_tc_kernel(const __grid_constant__ CUtensorMap map_cache, const 
             }
           }
         }
-        if (valid)
-          args.part_lse[static_cast<size_t>(args.part_first[token] + part) * args.hq + head] =
-              row_sum == 0.0f ? -INFINITY : top + log2f(row_sum);
+        if (valid) args.part_lse[part_row] = row_sum == 0.0f ? -INFINITY : top + log2f(row_sum);
       }
       named_barrier(1, 256);
       // whole rows of 512 bytes, a warp a row
       if (n_blocks > 0) {
-        for (int rr = warp - kShFirstSoftmaxWarp; rr < rows; rr += 8) {
-          const int pp = row0 + rr, to = members[pp / group];
-          const size_t at = static_cast<size_t>(args.part_first[to] + part) * args.hq + kv_head * group + pp % group;
-          *reinterpret_cast<float4*>(args.part_out + at * kShD + lane * 4) = *reinterpret_cast<const float4*>(exchange + rr * kShOutStride + lane * 4);
-        }
+#pragma unroll 4
+        for (int rr = warp - kShFirstSoftmaxWarp; rr < rows; rr += 8)
+          *reinterpret_cast<float4*>(args.part_out + static_cast<size_t>(part_rows[rr]) * kShD + lane * 4) =
+              *reinterpret_cast<const float4*>(exchange + rr * kShOutStride + lane * 4);
       }
     }
   }

@@ -690,7 +690,7 @@ def attention_lib(head_dim: int) -> ctypes.CDLL:
         lib.rl_attention_mma.restype = c_int
         lib.rl_attention_shared.argtypes = [
             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p,
-            c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p,
+            c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p,
             c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
         ]
         lib.rl_attention_shared.restype = c_int
@@ -898,7 +898,7 @@ def attention_shared(
             attention_lib(head_dim).rl_attention_shared(
                 _ptr(q), _ptr(cache), _ptr(out), _ptr(part_out), _ptr(part_lse), _ptr(tile_items), tile_items.numel() // SHARED_ITEM,
                 plan["tile_rows"], _ptr(row_items), row_items.numel() // SHARED_ITEM, plan["most_rows"], _ptr(members),
-                _ptr(positions), _ptr(part_first), _ptr(entry_slot), _ptr(block_table), tokens, num_heads, num_kv_heads, head_dim,
+                _ptr(positions), _ptr(part_first), plan["parts"], _ptr(entry_slot), _ptr(block_table), tokens, num_heads, num_kv_heads, head_dim,
                 cache.shape[3], cache.shape[0], block_table.shape[1], block_table.shape[0], float(scale), _ptr(sink), _ptr(slopes),
                 out_stride, _ptr(gate), gate_stride, _ptr(fault), int(PDL), _stream()),
             f"attention_shared(head_dim={head_dim})")

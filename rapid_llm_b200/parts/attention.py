@@ -263,7 +263,7 @@ class SharedItems(StepPlanner):
 
     # Measured times in microseconds by the rows of a tile: an item's start (page ids, queries, first keys, result), a block of 128
     # keys (64 in the float32 tiles of 32 rows), and how many items a multiprocessor runs at one time; the join of the parts: its start, a part, a part of 1,024 rows.
-    COSTS = {256: (7.0, 1.7, 1), 128: (6.0, 0.95, 1), 64: (4.0, 1.2, 2), 32: (5.0, 4.0, 2), 16: (3.0, 0.9, 3)}
+    COSTS = {256: (7.0, 1.7, 1), 128: (6.0, 0.95, 1), 64: (4.0, 1.2, 2), 32: (5.0, 4.0, 2), 16: (3.0, 0.9, 4)}
     JOIN = (2.0, 0.05, 0.35)
     STEPS = np.array([1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64, 96, 128, 192, 256, 512, 1024, 4096, 1 << 20])
 
