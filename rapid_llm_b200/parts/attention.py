@@ -262,36 +262,40 @@ class SharedItems(StepPlanner):
         return plan["parts"] * self.group * self.num_kv_heads
 
     # Measured times in microseconds by the rows of a tile: an item's start (page ids, queries, first keys, result), a block of 128
-    # keys (64 in the float32 tiles of 32 rows), and how many items a multiprocessor runs at one time; the join of the parts: its start, a part, a part of 1,024 rows.
-    COSTS = {256: (7.0, 1.7, 1), 128: (6.0, 0.95, 1), 64: (4.0, 1.2, 2), 32: (5.0, 4.0, 2), 16: (3.0, 0.9, 4)}
+    # keys (64 in the float32 tiles of 32 rows) of an item by itself, and how many items a multiprocessor runs at one time; the
+    # block of a row item when its neighbours stream too; the join of the parts: its start, a part, a part of 1,024 rows.
+    COSTS = {256: (7.0, 1.85, 1), 128: (6.0, 0.95, 1), 64: (4.0, 6.0, 3), 32: (5.0, 4.0, 2), 16: (5.0, 0.9, 4)}
+    STREAMED_BLOCK = 1.5
     JOIN = (2.0, 0.05, 0.35)
     STEPS = np.array([1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64, 96, 128, 192, 256, 512, 1024, 4096, 1 << 20])
 
     def _blocks_per_item(self, tiles, rows, tile_rows: int, tokens: int) -> tuple[int, int]:
         """Blocks of keys that a tile item and a row item take, for lists of (blocks, items side by side).  Short items fill the
         multiprocessors, but each has a start of its own and leaves a part of its rows' results to join.  A tile has a multiprocessor
-        to itself (its threads hold every register), so row items run on those that are left, and behind the tiles.  Of the
-        steps tried, the pair whose estimated end comes first."""
+        to itself (its threads hold every register), so row items run on those that are left, two on each, and what
+        finds no place there behind the tiles.  Of the steps tried, the pair whose estimated end comes first."""
         def of(kind, costs):
             start, block, together = costs
             if len(kind) == 0:
-                return np.array([1]), np.zeros(1), np.zeros(1), np.zeros(1), together
+                return np.array([1]), np.zeros(1), np.zeros(1), np.zeros(1), together, 0
             blocks, side = np.asarray(kind)[:, 0], np.asarray(kind)[:, 1]
             steps = self.STEPS[: int(np.searchsorted(self.STEPS, int(blocks.max()))) + 1]
             ranges = -(-blocks[None] // steps[:, None])
             end = start + block * np.minimum(steps[:, None], blocks[None]).max(1)
-            return steps, (ranges * side).sum(1), end, ranges.max(1), together
+            return steps, (ranges * side).sum(1), end, ranges.max(1), together, int((blocks * side).sum())
 
-        tile_steps, tile_items, tile_end, tile_parts, tile_together = of(tiles, self.COSTS[tile_rows])
-        row_steps, row_items, row_end, row_parts, row_together = of(rows, self.COSTS[kernels.DECODE_TILE_ROWS])
+        tile_steps, tile_items, tile_end, tile_parts, tile_together, _ = of(tiles, self.COSTS[tile_rows])
+        row_steps, row_items, row_end, row_parts, row_together, row_blocks = of(rows, self.COSTS[kernels.DECODE_TILE_ROWS])
         tile_items, tile_end, tile_parts = tile_items[:, None], tile_end[:, None], tile_parts[:, None]
-        tile_slots, slots = self.sms * tile_together, self.sms * row_together
-        tiles_done = np.ceil(tile_items / tile_slots) * tile_end
-        left = np.maximum(self.sms - tile_items / tile_together, 0) * row_together
-        beside = left * np.where(row_end > 0, np.maximum(np.floor(tiles_done / np.maximum(row_end, 1e-9)), tile_items == 0), 0)
-        behind = np.ceil(np.maximum(row_items - beside, 0) / slots)
+        tiles_done = np.ceil(tile_items / (self.sms * tile_together)) * tile_end
+        left = np.maximum(self.sms - tile_items / tile_together, 0)
+        row_work = row_items * (self.COSTS[kernels.DECODE_TILE_ROWS][0] / row_together) + row_blocks * self.STREAMED_BLOCK
+        # the last items' share of the time behind: streaming beside three others, a block takes as many times as long
+        longest = np.minimum(row_steps, int(np.asarray(rows)[:, 0].max())) if len(rows) else np.zeros(1)
+        behind = np.maximum(row_work - 0.8 * left * tiles_done, 0) / self.sms + 0.25 * (5.0 + self.STREAMED_BLOCK * row_together * longest)
+        behind = np.where(row_items <= 2 * left, 0.0, np.maximum(behind, row_end))
         parts = tile_parts + row_parts
-        end = np.maximum(tiles_done, np.where(beside > 0, row_end, 0.0)) + behind * row_end
+        end = np.maximum(tiles_done, np.where(left > 0, row_end, 0.0)) + behind
         end = end + self.JOIN[0] + self.JOIN[1] * parts + self.JOIN[2] * parts * (tokens * self.group * self.num_kv_heads / 1024)
         end = np.where((tile_items > 60000 * self.num_kv_heads) | (row_items > 60000 * self.num_kv_heads), np.inf, end)
         at = np.unravel_index(int(np.argmin(end)), end.shape)
@@ -366,17 +370,22 @@ class SharedItems(StepPlanner):
                 "heads": (self.group, self.num_kv_heads, self.head_dim), "dtype": self.tag}
 
     def saved_bytes(self, shape: StepShape) -> int:
-        """Bytes of keys and values that the members of the step's groups would read again if each read its own."""
+        """Bytes of keys and values that the members of the step's groups would read again if each read its own; groups of few
+        members, whose prefixes the ordinary kernels read as fast, do not count."""
         groups, shared = np.asarray(shape.prefix_group, dtype=np.int64), np.asarray(shape.prefix_tokens, dtype=np.int64)
         _, first, count = np.unique(groups, return_index=True, return_counts=True)
-        again = int(((count - 1) * shared[first] * (groups[first] >= 0)).sum())
+        counts = (groups[first] >= 0) & (count >= (2 if self.wide else MEMBERS_WORTH_SHARING))
+        again = int(((count - 1) * shared[first] * counts).sum())
         return again * 2 * self.num_kv_heads * self.head_dim * (4 if self.wide else 2)
 
     def step_plan(self, shape: StepShape) -> dict | None:
         """The plan of a decode-only step where sharing is worth its launches, else ``None``.  The lists are filled up with empty
         items and the number of parts is rounded up, to powers of two: what a captured step has baked in then changes at few
         context lengths."""
-        if not shape.decode_only or shape.prefix_group is None or self.saved_bytes(shape) < (WORTH_SHARING_F32 if self.wide else WORTH_SHARING):
+        if not shape.decode_only or shape.prefix_group is None:
+            return None
+        saved = self.saved_bytes(shape)
+        if saved == 0 or saved < (WORTH_SHARING_F32 if self.wide else WORTH_SHARING):
             return None
         plan = self.plan(shape)
         up = lambda n: 0 if n == 0 else 1 << (int(n) - 1).bit_length()
@@ -393,11 +402,14 @@ class SharedItems(StepPlanner):
         return 8 * (2048 + 8 * max_entries) + 3 * max_entries + 64
 
 
-# Bytes of keys and values, read again by every member but one, from which on a decode step reads shared prefixes once.  Measured
-# with 8 key heads of 128 and groups of 4 in bfloat16, us in a captured step, ordinary against shared, at requests x shared positions:
-# 8 x 1,024 (29 MB) 10.9 and 11.6, 4 x 4,096 (50 MB) 14.1 and 13.5, 32 x 512 (65 MB) 12.3 and 13.6, 2 x 16,384 (67 MB) 23.4 and
-# 25.9, 8 x 4,096 (117 MB) 20.2 and 15.8, 16 x 2,048 (126 MB) 17.8 and 13.2, 64 x 1,024 (264 MB) 36 and 23, 8 x 16,384 (470 MB) 62 and 25.
-WORTH_SHARING = 96 << 20
+# Bytes of keys and values, read again by every member but one of groups with so many members, from which on a decode step reads
+# shared prefixes once.  Measured with 8 key heads of 128 and groups of 4 in bfloat16, us in a captured step, ordinary against shared,
+# at requests x shared positions: 2 x 1,024 8.0 and 7.9, 2 x 16,384 (67 MB) 23.4 and 26.9, 4 x 1,024 (13 MB) 9.4 and 9.6, 4 x 4,096
+# (50 MB) 14.1 and 14.5, 8 x 256 (7 MB) 8.7 and 7.9, 8 x 1,024 (29 MB) 10.8 and 9.0, 8 x 4,096 20.2 and 15.8, 8 x 16,384 62 and 20,
+# 16 x 512 (31 MB) 8.8 and 8.5, 16 x 2,048 17.8 and 10.6, 32 x 512 (65 MB) 12.3 and 10.4, 64 x 256 (66 MB) 18.9 and 13.3, 64 x 1,024 36 and 18,
+# 64 x 8,192 220 and 40.
+WORTH_SHARING = 12 << 20
+MEMBERS_WORTH_SHARING = 5
 # ... and in float32, where the other kernel gives every row a warp of its own: 8 heads in groups of 4, 2 x 64 (0.02 MB) 22 and 8 us,
 # 8 x 128 39 and 11, 8 x 2,048 566 and 13.
 WORTH_SHARING_F32 = 0

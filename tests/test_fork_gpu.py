@@ -25,6 +25,7 @@ def sharing(request, monkeypatch):
 
     for name in ("WORTH_SHARING", "WORTH_SHARING_F32"):
         monkeypatch.setattr(attention, name, 0 if request.param else 1 << 62)
+    monkeypatch.setattr(attention, "MEMBERS_WORTH_SHARING", 2)
     return request.param
 
 

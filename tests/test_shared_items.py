@@ -84,3 +84,38 @@ def test_there_is_no_cpu_path():
         kernels.attention_shared(torch.zeros((1, 64)), torch.zeros((2, 2, 1, 16, 64)), torch.zeros((1, 64)), plan={}, part_out=None, part_lse=None,
                                  positions=torch.zeros(1, dtype=torch.int32), cu_seqlens=None, entry_start=None, entry_slot=None,
                                  block_table=None, num_heads=1, num_kv_heads=1, head_dim=64, scale=1.0, fault=None)
+
+
+def test_the_rule_of_a_decode_step():
+    """Shared where that saves enough for groups of enough members; lists filled up to powers of two; never in steps with portions."""
+    from rapid_llm_b200.parts import attention
+
+    items = SharedItems(4, 8, 128)
+    def shape(members, prefix, own=5, lengths=None):
+        return shape_of(lengths or [1] * members, [prefix + own] * members, [3] * members, [prefix] * members)
+
+    per_position = 2 * 8 * 128 * 2
+    assert items.saved_bytes(shape(8, 1000)) == 7 * 1000 * per_position and items.saved_bytes(shape(4, 1000)) == 0
+    edge = -(-attention.WORTH_SHARING // (7 * per_position))
+    assert items.step_plan(shape(8, edge)) is not None and items.step_plan(shape(8, edge - 1)) is None
+    assert items.step_plan(shape(4, 100_000)) is None and items.step_plan(shape(8, 5000, lengths=[1] * 7 + [2])) is None
+    wide = SharedItems(4, 8, 128, dtype=torch.float32)
+    assert wide.step_plan(shape(2, 16)) is not None and wide.step_plan(shape(1, 16)) is None and wide.step_plan(shape(2, 0)) is None
+    plan = items.step_plan(shape(11, 5000, 300))
+    assert plan["shared"] is True
+    for name in ("tile_items", "row_items"):
+        count = len(plan[name])
+        assert count & (count - 1) == 0 and (plan[name][plan[name][:, 5] == 0] == 0).all()
+    assert plan["parts"] & (plan["parts"] - 1) == 0 and plan["parts"] >= plan["part_first"][-1]
+    counts = {tuple((k, len(v) if isinstance(v, np.ndarray) else v) for k, v in items.step_plan(shape(11, 5000, own)).items()) for own in range(1, 400)}
+    assert len(counts) <= 6                  # what a captured step has baked in, over 400 steps
+
+
+def test_the_lists_fit_what_the_planner_asks_for():
+    for members in (5, 33, 64):
+        for prefix in (200, 5000, 200_000):
+            items = SharedItems(4, 1, 128)
+            plan = items.step_plan(shape_of([1] * members, [prefix + 9000] * members, [0] * members, [prefix] * members))
+            if plan is not None:
+                size = sum(v.size + 3 for v in plan.values() if isinstance(v, np.ndarray))
+                assert size <= items.capacity(members, members)
