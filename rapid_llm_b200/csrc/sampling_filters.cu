@@ -214,6 +214,20 @@ struct Row {
     return one[0];
   }
 
+  // Every token of the slice once, in any order: 16 bytes a load.
+  template <typename Fn>
+  __device__ __forceinline__ void sweep_any(Fn&& fn) {
+    constexpr int kWide = 16 / sizeof(Store);
+    const int whole = count / kWide * kWide;
+    for (int i0 = threadIdx.x * kWide; i0 < whole; i0 += kThreads * kWide) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(values + i0);
+      const Store* several = reinterpret_cast<const Store*>(&raw);
+#pragma unroll
+      for (int k = 0; k < kWide; ++k) fn(i0 + k, to_float(several[k]));
+    }
+    if (whole + threadIdx.x < count) fn(whole + threadIdx.x, to_float(values[whole + threadIdx.x]));
+  }
+  // A thread's tokens side by side, so that the threads' sums are in index order.
   template <typename Fn>
   __device__ __forceinline__ void sweep(Fn&& fn) {
     const int first = min(count, static_cast<int>(threadIdx.x) * chunk), last = min(count, first + chunk);
@@ -245,7 +259,7 @@ struct Row {
     }
     __syncthreads();
     const float back = 1.0f / code_scale, scale2 = static_cast<float>(per * (1.0 / 64.0));
-    sweep([&](int i, float x) {
+    sweep_any([&](int i, float x) {
       const unsigned q = code(x);
       if (q < at.low || q > at.high || !in(i, x)) return;
       const unsigned b = (q - at.low) >> shift;
@@ -366,7 +380,7 @@ struct Row {
   __device__ unsigned gather(unsigned low, unsigned high, In&& in) {
     if (threadIdx.x == 0) s.list_n = 0;
     __syncthreads();
-    sweep([&](int i, float x) {
+    sweep_any([&](int i, float x) {
       const unsigned q = code(x);
       if (q < low || q > high || !in(i, x)) return;
       const unsigned place = atomicAdd(&s.list_n, 1u);
@@ -398,7 +412,7 @@ struct Row {
   template <typename In>
   __device__ void range_of(const Interval& at, In&& in, float& most, float& least) {
     unsigned high = 0, low = 0;
-    sweep([&](int i, float x) {
+    sweep_any([&](int i, float x) {
       const unsigned q = code(x);
       if (q < at.low || q > at.high || !in(i, x)) return;
       high = max(high, ordered(x));
@@ -637,18 +651,18 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       while (a < b) {
         const unsigned mid = a + (b - a) / 2;
         u64 n = 0;
-        row.sweep([&](int, float v) { n += ordered(v) > mid; });
+        row.sweep_any([&](int, float v) { n += ordered(v) > mid; });
         if (row.cluster_sum(n) >= static_cast<u64>(want_k)) a = mid + 1; else b = mid;
       }
       cut_k = unordered(a);
       u64 n = 0;
-      row.sweep([&](int, float v) { n += ordered(v) > a; });
+      row.sweep_any([&](int, float v) { n += ordered(v) > a; });
       const u64 ties = static_cast<u64>(want_k) - row.cluster_sum(n);    // of the equal ones so many stay
       int from = 0, to = args.vocab - 1;
       while (from < to) {
         const int mid = from + (to - from) / 2;
         n = 0;
-        row.sweep([&](int i, float v) { n += ordered(v) == a && row.begin + i <= mid; });
+        row.sweep_any([&](int i, float v) { n += ordered(v) == a && row.begin + i <= mid; });
         if (row.cluster_sum(n) >= ties) to = mid; else from = mid + 1;
       }
       cut_i = from;
@@ -720,7 +734,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       while (at.inside_n > kList && at.low < at.high) {
         const unsigned mid = at.low + (at.high - at.low) / 2;
         u64 near_mass = 0, near_n = 0;
-        row.sweep([&](int i, float v) {
+        row.sweep_any([&](int i, float v) {
           const unsigned q = row.code(v);
           if (q < at.low || q > mid || !in_k(i, v)) return;
           near_mass += row.weight(v);
@@ -759,7 +773,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
         while (a < b) {
           const unsigned mid = a + (b - a) / 2;
           u64 mass = 0;
-          row.sweep([&](int i, float v) {
+          row.sweep_any([&](int i, float v) {
             if (ordered(v) > mid && row.code(v) >= at.low && in_k(i, v)) mass += row.weight(v);
           });
           if (static_cast<double>(above + row.cluster_sum(mass)) <= budget) b = mid; else a = mid + 1;
