@@ -74,15 +74,31 @@ def _need_cuda(*tensors: torch.Tensor | None) -> None:
             )
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _here(tensor: torch.Tensor) -> int:
+    """The current device, which the tensor has to live on: the launch goes to that one's stream."""
+    if not tensor.is_cuda:
+        _need_cuda(tensor)
+    here = _current_device()
+    if tensor.get_device() != here:
+        raise KernelError(f"kernel arguments must live on the current device (cuda:{here}), got a tensor on {tensor.device}")
+    return here
+
+
 def _need_here(*tensors: torch.Tensor | None) -> None:
-    """Every tensor on the current device, whose stream the launch goes to."""
     here = None
     for tensor in tensors:
         if tensor is not None and tensor.get_device() != here:
-            _need_cuda(tensor)
-            here = torch.cuda.current_device()
-            if tensor.get_device() != here:
-                raise KernelError(f"kernel arguments must live on the current device (cuda:{here}), got a tensor on {tensor.device}")
+            here = _here(tensor)
+
+
+def _need_list(name: str, tensor: torch.Tensor, dtype: torch.dtype, here: int) -> int:
+    """The address of a contiguous array of ``dtype`` on device ``here``."""
+    if tensor.dtype is not dtype or tensor.get_device() != here or not tensor.is_contiguous():
+        _here(tensor), _expect(name, tensor, dtype), _contig(name, tensor)
+    return tensor.data_ptr()
 
 
 def _contig(name: str, tensor: torch.Tensor | None) -> None:
@@ -274,15 +290,15 @@ def copy_pages(pages: torch.Tensor, pairs) -> torch.Tensor:
     if pairs.dtype.kind not in "iu" or pairs.ndim != 2 or pairs.shape[1] != 2:
         raise KernelError("copy_pages: pairs must be integers [n, 2]")
     listed = np.ascontiguousarray(pairs, dtype=np.int32)
-    if pairs.dtype.itemsize > 4 and (listed != pairs).any():
+    if pairs.dtype != np.int32 and (listed != pairs).any():
         raise KernelError("copy_pages: a page's number does not fit 32 bits")
-    count, known, lib = listed.shape[0], pages.shape[1], core()
-    broken = lib.rl_copy_pages_check(listed.ctypes.data, count, known)
+    count, known, lib, listed_at = listed.shape[0], pages.shape[1], core(), listed.__array_interface__["data"][0]
+    broken = lib.rl_copy_pages_check(listed_at, count, known)
     if broken:
         raise KernelError("copy_pages: " + {-1: f"a pair names a page outside the {known} there are",
                                             -2: "a page is written twice, or both read and written"}.get(broken, "no host memory"))
     size = pages.element_size()
-    _check(lib.rl_copy_pages(_ptr(pages), listed.ctypes.data, count, pages.shape[0], pages.stride(0) * size,
+    _check(lib.rl_copy_pages(_ptr(pages), listed_at, count, pages.shape[0], pages.stride(0) * size,
                              pages.stride(1) * size, int(PDL), _stream()), "copy_pages")
     LAUNCHES.count += lib.rl_copy_pages_launches(count) - 1
     return pages
@@ -855,53 +871,44 @@ def attention_shared(
     ``[part_rows, head_dim]`` and ``part_lse`` ``[part_rows]`` (float32) are scratch of ``SharedItems.part_rows(plan)`` rows
     and more; calls that may run at the same time need scratch of their own.  ``sink``, ``gate`` and ``slopes`` as in :func:`attention_mma`, rows of ``out`` and
     ``gate`` too; every key up to a token's own position is seen (no window, no squashed scores, caches of two planes)."""
-    _need_here(q, cache, out, part_out, part_lse, positions, cu_seqlens, entry_start, entry_slot, block_table, fault, sink, gate, slopes)
-    _per_head(num_heads, sink=sink, slopes=slopes)
-    _contig("q", q), _contig("cache", cache)
-    for name, tensor in (("positions", positions), ("cu_seqlens", cu_seqlens), ("entry_start", entry_start),
-                         ("entry_slot", entry_slot), ("block_table", block_table), ("fault", fault)):
-        _expect(name, tensor, torch.int32), _contig(name, tensor)
-    tokens, width = positions.numel(), num_heads * head_dim
-    if cache.dim() != 5 or cache.shape[1] != 2 or cache.shape[2] != num_kv_heads or cache.shape[4] != head_dim or num_heads % num_kv_heads:
+    here, dtype = _here(q), q.dtype
+    q_at, cache_at = _need_list("q", q, dtype, here), _need_list("cache", cache, dtype, here)
+    at = [_need_list(name, tensor, torch.int32, here) for name, tensor in (
+        ("positions", positions), ("entry_slot", entry_slot), ("block_table", block_table), ("fault", fault),
+        ("tile_items", plan["tile_items"]), ("row_items", plan["row_items"]), ("members", plan["members"]), ("part_first", plan["part_first"]),
+        ("cu_seqlens", cu_seqlens), ("entry_start", entry_start))]
+    tokens, shape = positions.shape[0] if positions.dim() == 1 else positions.numel(), cache.shape
+    if len(shape) != 5 or shape[1] != 2 or shape[2] != num_kv_heads or shape[4] != head_dim or num_heads % num_kv_heads:
         raise KernelError("attention: cache must be [pages, 2, kv_heads, page_size, head_dim], heads a multiple of kv heads")
-    if q.shape != (tokens, width) or out.shape != q.shape or cache.dtype != q.dtype or out.dtype != q.dtype:
+    if q.shape != (tokens, num_heads * head_dim) or out.shape != q.shape or out.dtype is not dtype or out.get_device() != here:
         raise KernelError("attention: q and out must be [tokens, heads * head_dim] of the cache's dtype")
-    if plan["tokens"] != tokens or plan["heads"] != (num_heads // num_kv_heads, num_kv_heads, head_dim) or plan["dtype"] != dtype_tag(q.dtype):
+    if plan["tokens"] != tokens or plan["heads"] != (num_heads // num_kv_heads, num_kv_heads, head_dim) or plan["dtype"] != dtype_tag(dtype):
         raise KernelError("attention: the plan was made for another step")
     if not scale > 0:
         raise KernelError("attention: the scale must be positive")
     if plan["entries"] != entry_slot.numel() or block_table.dim() != 2:
         raise KernelError("attention: the plan was made for another number of entries")
+    if sink is not None or slopes is not None or gate is not None:
+        _need_here(q, sink, slopes, gate)
+        _per_head(num_heads, sink=sink, slopes=slopes)
     out_stride, gate_stride = _attention_out(out, gate, tokens, num_heads, head_dim)
-    tile_items, row_items = plan["tile_items"], plan["row_items"]
-    members, part_first = plan["members"], plan["part_first"]
-    _need_here(tile_items, row_items, members, part_first)
-    for name, tensor in (("tile_items", tile_items), ("row_items", row_items), ("members", members), ("part_first", part_first)):
-        _expect(name, tensor, torch.int32), _contig(name, tensor)
-    need = plan["parts"] * num_heads
-    _expect("part_out", part_out, torch.float32), _expect("part_lse", part_lse, torch.float32)
-    if part_out is None or part_lse is None or part_out.numel() < need * head_dim or part_lse.numel() < need:
+    parts = plan["parts"]
+    if part_out is None or part_lse is None or part_out.numel() < parts * num_heads * head_dim or part_lse.numel() < parts * num_heads:
         raise KernelError("attention: scratch for the parts is missing or too small")
-    _contig("part_out", part_out), _contig("part_lse", part_lse)
-    if q.dtype == torch.float32:
-        launches = 1 + (tile_items.numel() > 0)
-        _check(
-            core().rl_attention_shared_f32(
-                _ptr(q), _ptr(cache), _ptr(out), _ptr(part_out), _ptr(part_lse), _ptr(tile_items), tile_items.numel() // SHARED_ITEM,
-                _ptr(members), _ptr(positions), _ptr(part_first), _ptr(entry_slot), _ptr(block_table), tokens, num_heads,
-                num_kv_heads, head_dim, cache.shape[3], cache.shape[0], block_table.shape[1], block_table.shape[0], float(scale),
-                _ptr(sink), _ptr(slopes), out_stride, _ptr(gate), gate_stride, _ptr(fault), int(PDL), _stream()),
-            f"attention_shared(head_dim={head_dim})")
+    scratch = _need_list("part_out", part_out, torch.float32, here), _need_list("part_lse", part_lse, torch.float32, here)
+    positions_at, slot_at, table_at, fault_at, tiles_at, rows_at, members_at, first_at, _, _ = at
+    tiles, rows = plan["tile_items"].shape[0], plan["row_items"].shape[0]
+    what = (tokens, num_heads, num_kv_heads, head_dim, shape[3], shape[0], block_table.shape[1], block_table.shape[0], float(scale),
+            _ptr(sink), _ptr(slopes), out_stride, _ptr(gate), gate_stride, fault_at, int(PDL), _stream())
+    if dtype is torch.float32:
+        launches = 1 + (tiles > 0)
+        _check(core().rl_attention_shared_f32(q_at, cache_at, out.data_ptr(), *scratch, tiles_at, tiles, members_at, positions_at, first_at,
+                                              slot_at, table_at, *what), "attention_shared")
     else:
-        launches = 1 + (tile_items.numel() > 0) + (row_items.numel() > 0)
-        _check(
-            attention_lib(head_dim).rl_attention_shared(
-                _ptr(q), _ptr(cache), _ptr(out), _ptr(part_out), _ptr(part_lse), _ptr(tile_items), tile_items.numel() // SHARED_ITEM,
-                plan["tile_rows"], _ptr(row_items), row_items.numel() // SHARED_ITEM, plan["most_rows"], _ptr(members),
-                _ptr(positions), _ptr(part_first), plan["parts"], _ptr(entry_slot), _ptr(block_table), tokens, num_heads, num_kv_heads, head_dim,
-                cache.shape[3], cache.shape[0], block_table.shape[1], block_table.shape[0], float(scale), _ptr(sink), _ptr(slopes),
-                out_stride, _ptr(gate), gate_stride, _ptr(fault), int(PDL), _stream()),
-            f"attention_shared(head_dim={head_dim})")
+        launches = 1 + (tiles > 0) + (rows > 0)
+        _check(attention_lib(head_dim).rl_attention_shared(
+            q_at, cache_at, out.data_ptr(), *scratch, tiles_at, tiles, plan["tile_rows"], rows_at, rows, plan["most_rows"], members_at,
+            positions_at, first_at, parts, slot_at, table_at, *what), "attention_shared")
     LAUNCHES.count += launches - 1
     return out
 
