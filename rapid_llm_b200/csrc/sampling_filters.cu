@@ -14,10 +14,14 @@
 // 2^-44 round to zero; only u = 0, which takes the first index that stays, can meet one, and looks at float64 itself.
 //
 // A row is spread over a thread-block cluster and lies in its shared memory.  The cuts are found on linear codes of
-// the distance to the maximum (23 bits, monotone): histograms of 256 bins over the interval that holds the cut, with exact counts
-// for top-k and masses to 2^-15 of themselves for top-p, narrow the interval until it holds at most 256 tokens, a
+// the distance to the maximum (23 bits, monotone): histograms of 256 bins over the interval that holds the cut, with exact
+// counts for top-k and masses to 2^-15 of themselves for top-p, narrow the interval until it holds at most 256 tokens, a
 // single value, or the whole top-k; then the tokens of the interval are compared with one another, exactly.  Intervals
 // that end otherwise (more than 256 tokens of different values within 2^-23 of the range) are cut by bisection with exact sums.
+//
+// Bound by the chain of steps in a row, each a sweep of shared memory, a barrier of the cluster and a look at 256 bins (2 to
+// 3 us): 15 us for one row of 151,936 with top-k 50, 51 for 32 float32 rows that only top-p cuts, whose exact sums (about
+// 11 us each, float64 exponentials) come on top, 24 for 256 rows of 32,003 with top-k; the logits alone are 0.05 to 3 us.
 #include "common.cuh"
 
 namespace rl {
@@ -31,6 +35,9 @@ constexpr int kMaxRanks = 8;
 constexpr int kMaxSlice = 48 * 1024;          // numbers of one CTA's slice (192 KB as floats)
 constexpr int kCodeBits = 23;
 constexpr double kUnit = 8796093022208.0;     // 2^43: a weight of one
+// What mass(before) - p * mass(all) can be off by where histograms give both, as a share of the whole.  A token's part of its bin's
+// edge is off by 2^-16 at most and is 0.61 at least (64 bins or more span 31 nats), its float32 distance costs 4e-6: 2.9e-5 each.
+constexpr double kSlack = 6e-5;
 constexpr float kNegligible = 31.0f;          // (m - x) / T beyond which a weight rounds to zero (44 ln 2 = 30.5)
 using u64 = unsigned long long;
 
@@ -248,13 +255,14 @@ struct Row {
 
   // One step: histogram of the interval's codes (and masses), the bins that hold the cut become the interval.
   // kMass false: the cut is the token of rank `want` (counted from 0); true: `share_of` times the whole mass.
-  template <bool kMass, typename In>
+  // kCount: counts are taken (without them a bin holds a token if it holds mass, and how many the interval holds is not known).
+  template <bool kMass, bool kCount, typename In>
   __device__ void narrow(Interval& at, unsigned want, double share_of, double& whole, In&& in) {
     const unsigned span = at.high - at.low;
     const int shift = max(0, 24 - __clz(span));           // (span >> shift) < 256
     const int buffer = level++ & 1;
     for (int b = threadIdx.x; b < kBins; b += kThreads) {
-      s.bins[buffer][b] = 0;
+      if (kCount) s.bins[buffer][b] = 0;
       if (kMass) s.mass[buffer][b] = 0;
     }
     __syncthreads();
@@ -263,7 +271,7 @@ struct Row {
       const unsigned q = code(x);
       if (q < at.low || q > at.high || !in(i, x)) return;
       const unsigned b = (q - at.low) >> shift;
-      atomicAdd(&s.bins[buffer][b], 1u);
+      if (kCount) atomicAdd(&s.bins[buffer][b], 1u);
       if (kMass) {
         // relative to the bin's upper edge: 16 bits whatever the mass
         const float edge = static_cast<float>(at.low + (b << shift)) * back;
@@ -277,11 +285,11 @@ struct Row {
       unsigned n = 0;
       double m = 0.0;
       for (unsigned r = 0; r < ranks; ++r) {
-        n += ranks == 1 ? s.bins[buffer][b] : peer_u32(&s.bins[buffer][b], r);
+        if (kCount) n += ranks == 1 ? s.bins[buffer][b] : peer_u32(&s.bins[buffer][b], r);
         if (kMass) m += static_cast<double>(ranks == 1 ? s.mass[buffer][b] : peer_u32(&s.mass[buffer][b], r));
       }
-      s.counts[b] = n;
-      if (kMass) s.total[b] = m * exp2(-static_cast<double>(at.low + (static_cast<unsigned>(b) << shift)) * back * (per * (1.0 / 64.0)));
+      s.counts[b] = kCount ? n : m > 0.0;
+      if (kMass) s.total[b] = m * (1.0 / 32768.0) * exp2(-static_cast<double>(at.low + (static_cast<unsigned>(b) << shift)) * back * (per * (1.0 / 64.0)));
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -312,7 +320,7 @@ struct Row {
       if (kMass && whole < 0.0) whole = __shfl_sync(0xffffffffu, at.above + upto_mass, 31);
       // first and last bin the cut can lie in
       int low = -1, high = -1;
-      const double budget = share_of * whole, slack = 4e-5 * whole;
+      const double budget = share_of * whole, slack = kSlack * whole;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (n[i] > 0) {
@@ -374,9 +382,10 @@ struct Row {
     __syncthreads();
   }
 
-  // Tokens of the cluster with codes low .. high (at most kList of them) into all_x, all_i, all_w of every CTA; returns how
-  // many.  A rank's list may be written again only behind a barrier of the cluster (no call gathers twice without one).
-  template <typename In>
+  // Tokens of the cluster with codes low .. high (at most kList of them) into all_x, all_i, all_w of every CTA (kFirstOnly: of
+  // the first, the others go on); returns how many.  A rank's list may be written again only behind a barrier of the cluster
+  // (no call gathers twice without one).
+  template <bool kFirstOnly, typename In>
   __device__ unsigned gather(unsigned low, unsigned high, In&& in) {
     if (threadIdx.x == 0) s.list_n = 0;
     __syncthreads();
@@ -391,6 +400,7 @@ struct Row {
     });
     __syncthreads();
     if (ranks > 1) cluster_barrier();
+    if (kFirstOnly && rank != 0) return 0;
     if (threadIdx.x < ranks) s.list_of[threadIdx.x] = ranks == 1 ? s.list_n : peer_u32(&s.list_n, threadIdx.x);
     __syncthreads();
     unsigned all = 0;
@@ -463,12 +473,15 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   const bool vector = (reinterpret_cast<uintptr_t>(x) & (sizeof(T) == 2 ? 15 : 31)) == 0;
   const int vector_count = vector ? (row.count & ~7) : 0;
   auto clean = [](float v) { return v == v ? v + 0.0f : -INFINITY; };      // (the sum makes a negative zero the zero it equals)
-  // the largest value with the first index it has (as a complement), and the smallest finite one, on the way
-  u64 ends[2] = {0ull, 0ull};
+  // the largest value with the first index it has (a thread meets its own in rising order), and the smallest finite one, on the way
+  float most = -INFINITY, least = INFINITY;
+  int most_at = -1;
   auto seen = [&](int i, float v) {
-    const unsigned k = ordered(v);
-    ends[0] = max(ends[0], static_cast<u64>(k) << 32 | ~static_cast<unsigned>(row.begin + i));
-    if (v > -INFINITY) ends[1] = max(ends[1], static_cast<u64>(~k));
+    if (v > most) {
+      most = v;
+      most_at = i;
+    }
+    least = v > -INFINITY ? fminf(least, v) : least;
   };
   const bool penalised = pen != 1.0f && args.seen_tokens != nullptr && seen_end > seen_begin;
   constexpr int kFly = sizeof(T) == 2 ? 5 : 3;       // 8-element loads of a thread in flight, kept as they come
@@ -521,15 +534,17 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
     __syncthreads();
     row.sweep(seen);
   }
+  u64 ends[2] = {most_at < 0 ? 0ull : static_cast<u64>(ordered(most)) << 32 | ~static_cast<unsigned>(row.begin + most_at),
+                 least == INFINITY ? 0ull : static_cast<u64>(~ordered(least))};
   row.template cluster_all<typename R::Most>(ends);
-  float top = unordered(static_cast<unsigned>(ends[0] >> 32));
-  if (ends[0] == 0ull || !(top > -INFINITY) || !(temp > 0.0f)) {
+  float top = ends[0] == 0ull ? -INFINITY : unordered(static_cast<unsigned>(ends[0] >> 32));
+  if (!(top > -INFINITY) || !(temp > 0.0f)) {
     // nothing to choose from, or the first maximum; nobody leaves while its shared memory may be read
     if (row.rank == 0 && threadIdx.x == 0) args.out[row_index] = top > -INFINITY ? static_cast<int>(~static_cast<unsigned>(ends[0])) : 0;
     if (ranks > 1) cluster_barrier();
     return;
   }
-  float bottom = unordered(~static_cast<unsigned>(ends[1]));
+  float bottom = ends[1] == 0ull ? top : unordered(~static_cast<unsigned>(ends[1]));
   if (top == INFINITY) {                             // entries of +infinity share everything
     row.sweep([&](int i, float v) { slice_values[i] = from_float<Store>(v == INFINITY ? 0.0f : -INFINITY); });
     top = bottom = 0.0f;
@@ -578,7 +593,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
     double unused = 0.0;
     bool fewer = false;
     for (bool first = true;; first = false) {
-      row.template narrow<false>(at, static_cast<unsigned>(want_k - 1), 0.0, unused, everything);
+      row.template narrow<false, true>(at, static_cast<unsigned>(want_k - 1), 0.0, unused, everything);
       if (first) {
         // fewer tokens than k that can be drawn at all: the others weigh nothing, every one may stay
         fewer = s.whole_n <= static_cast<unsigned>(want_k);
@@ -589,8 +604,12 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       // nothing is cut
     } else if (at.above_n + at.inside_n <= kList) {
       // the whole of top-k and a little more fits the list: everything else happens there
-      const unsigned n = row.gather(0u, at.high, everything);
-      // (the same in every CTA).  Each token is compared with all others by `side` neighbouring lanes.
+      const unsigned n = row.template gather<true>(0u, at.high, everything);
+      if (row.rank != 0) {
+        cluster_barrier();                           // the first CTA may still read this one's list
+        return;
+      }
+      // Each token is compared with all others by `side` neighbouring lanes.
       const unsigned padded = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256, side = kThreads / padded;
       const unsigned mine = threadIdx.x / side, sub = threadIdx.x % side;
       const bool have = mine < n, lead = sub == 0;
@@ -621,14 +640,14 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       for (unsigned j = sub; j < n; j += side)
         before += s.all_keep[j] && s.all_i[j] < my_i ? (first_of_all ? 1ull : s.all_w[j]) : 0ull;
       before = over_side(before);
-      if (keep && lead && row.rank == 0) {
+      if (keep && lead) {
         const u64 target = first_of_all ? 0ull : target_of(mass);
         if (before <= target && target < before + (first_of_all ? 1ull : my_w)) args.out[row_index] = my_i;
       }
       if (ranks > 1) cluster_barrier();
       return;
     } else if (at.inside_n <= kList) {
-      const unsigned n = row.gather(at.low, at.high, everything);
+      const unsigned n = row.template gather<false>(at.low, at.high, everything);
       if (threadIdx.x < n) {
         const float my_x = s.all_x[threadIdx.x];
         const int my_i = s.all_i[threadIdx.x];
@@ -677,8 +696,9 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   if (by_mass) {
     typename R::Interval at = {0u, kLast, 0u, 0u, 0.0};
     double whole = -1.0;
-    for (int level = 0; level < 3; ++level) {
-      row.template narrow<true>(at, 0u, fmax(static_cast<double>(p), 0.0), whole, in_k);
+    row.template narrow<true, false>(at, 0u, fmax(static_cast<double>(p), 0.0), whole, in_k);
+    for (int level = 0; level < 2; ++level) {
+      row.template narrow<true, true>(at, 0u, fmax(static_cast<double>(p), 0.0), whole, in_k);
       if (at.inside_n <= kList || at.low == at.high) break;
     }
     float high, low;
@@ -686,7 +706,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
     if (at.inside_n > kList) {
       row.range_of(at, in_k, high, low);
     } else {
-      listed = row.gather(at.low, at.high, in_k);
+      listed = row.template gather<false>(at.low, at.high, in_k);
       u64 ends_of[2] = {0ull, 0ull};
       if (threadIdx.x < listed) {
         ends_of[0] = ordered(s.all_x[threadIdx.x]);
@@ -706,9 +726,14 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
         const u64 w = row.weight(v);
         const unsigned q = row.code(v);
         z += w;
-        if (q < at.low) above += w;
-        else if (q <= at.high) inside += w;
-        else if (q <= kLast) behind += 1;
+        if (q < at.low) {
+          above += w;
+          behind += 1ull << 32;                        // (tokens before the interval ride in the upper half)
+        } else if (q <= at.high) {
+          inside += w;
+        } else if (q <= kLast) {
+          behind += 1;
+        }
       });
       u64 sums[4] = {z, above, inside, behind};
       row.template cluster_all<typename R::Sum>(sums);
@@ -717,16 +742,17 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       z = sums[0];
       above = sums[1];
       inside = sums[2];
-      behind = sums[3];
+      const unsigned front_n = static_cast<unsigned>(sums[3] >> 32);
+      behind = sums[3] & 0xffffffffull;
       const double budget = fmax(static_cast<double>(p), 0.0) * static_cast<double>(z);
       if (static_cast<double>(above) > budget) {       // (not met: the approximate masses are nearer than their slack)
-        at = {0u, at.low - 1u, 0u, at.above_n, 0.0};
+        at = {0u, at.low - 1u, 0u, front_n, 0.0};
         above = 0;
         weighed = 0;
         weighed_to = 0;
         listed = 0;
       } else if (static_cast<double>(above + inside) <= budget && behind > 0) {
-        at = {at.high + 1u, kLast, at.above_n + at.inside_n, static_cast<unsigned>(behind), 0.0};
+        at = {at.high + 1u, kLast, 0u, static_cast<unsigned>(behind), 0.0};
         above += inside;
         listed = 0;
       }
@@ -754,7 +780,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
         }
       }
       if (at.inside_n <= kList) {
-        const unsigned n = listed > 0 ? listed : row.gather(at.low, at.high, in_k);
+        const unsigned n = listed > 0 ? listed : row.template gather<false>(at.low, at.high, in_k);
         unsigned best = 0;                             // the smallest that stays, as the largest of the complements
         if (threadIdx.x < n) {
           const float my_x = s.all_x[threadIdx.x];
@@ -885,8 +911,9 @@ int rl_sample_filtered(int dtype, const void* logits, int rows, int vocab, long 
   const bool halves = dtype == rl::kBF16 && (penalty == nullptr || seen_tokens == nullptr);
   const int size = halves ? 2 : 4, slots = 2 * rl::filters::sm_count();
   // CTAs a row: as many as run at one time (two a multiprocessor), since a row's steps wait for one another more than they compute, as
-  // long as two slices fit.  With 8 and with fewer: 256 rows of 32,003 107 and 31 us (1), 64 rows of 151,936 with top-k 47 and
-  // 36 (4); that disagree about everything 78 and 82; one row 19 and 27.
+  // long as two slices fit.  In us with 8, 4, 2 and 1 (bfloat16): 256 rows of 32,003 with top-k 50 102, 55, 36, 25, without
+  // 185, 109, 82, 68; 64 rows 28, 16, 17, 19 and 53, 32, 36, 49; 64 rows of 151,936 38, 28 and 120, 103; one row 15, 19.
+  // Where most rows end early, the later ones start sooner in small pieces: 64 rows of which few are long 64 with 8, 80 with 4.
   int ranks = rl::filters::kMaxRanks;
   while (ranks > 1 && rows * ranks > slots && ((vocab + ranks / 2 - 1) / (ranks / 2) + 8) * size <= rl::filters::kRoomyBytes) ranks /= 2;
   rl::filters::Args a = {};
