@@ -800,20 +800,20 @@ static int launch_shared_tc(const AttentionArgs& a, int n_items, int tile_rows, 
   if constexpr (kDim != kTcD) {
     return static_cast<int>(cudaErrorInvalidValue);
   } else {
-  CUtensorMap map;
-  const long long rows = static_cast<long long>(a.num_pages) * 2 * a.hkv * a.page_size;
-  int status = make_map(&map, a.cache, rows, kD, a.page_size < kShKeys ? a.page_size : kShKeys);
-  if (status != 0) return status;
-  SharedTcArgs t = {};
-  t.q = a.q; t.part_out = a.part_out; t.part_lse = a.part_lse; t.items = a.items; t.entry_slot = a.entry_slot;
-  t.block_table = a.block_table; t.members = a.members; t.positions = a.positions; t.part_first = a.part_first;
-  t.hq = a.hq; t.hkv = a.hkv; t.page_size = a.page_size; t.num_pages = a.num_pages; t.max_pages = a.max_pages; t.slots = a.slots;
-  t.scale_log2 = a.scale_log2; t.slopes = a.slopes; t.fault = a.fault;
-  if (tile_rows == 2 * kShTileRows)
-    return a.slopes != nullptr ? launch_shared_tc_as<true, true>(map, t, n_items, pdl, stream)
-                               : launch_shared_tc_as<true, false>(map, t, n_items, pdl, stream);
-  return a.slopes != nullptr ? launch_shared_tc_as<false, true>(map, t, n_items, pdl, stream)
-                             : launch_shared_tc_as<false, false>(map, t, n_items, pdl, stream);
+    CUtensorMap map;
+    const long long rows = static_cast<long long>(a.num_pages) * 2 * a.hkv * a.page_size;
+    int status = make_map(&map, a.cache, rows, kD, a.page_size < kShKeys ? a.page_size : kShKeys);
+    if (status != 0) return status;
+    SharedTcArgs t = {};
+    t.q = a.q; t.part_out = a.part_out; t.part_lse = a.part_lse; t.items = a.items; t.entry_slot = a.entry_slot;
+    t.block_table = a.block_table; t.members = a.members; t.positions = a.positions; t.part_first = a.part_first;
+    t.hq = a.hq; t.hkv = a.hkv; t.page_size = a.page_size; t.num_pages = a.num_pages; t.max_pages = a.max_pages; t.slots = a.slots;
+    t.scale_log2 = a.scale_log2; t.slopes = a.slopes; t.fault = a.fault;
+    if (tile_rows == 2 * kShTileRows)
+      return a.slopes != nullptr ? launch_shared_tc_as<true, true>(map, t, n_items, pdl, stream)
+                                 : launch_shared_tc_as<true, false>(map, t, n_items, pdl, stream);
+    return a.slopes != nullptr ? launch_shared_tc_as<false, true>(map, t, n_items, pdl, stream)
+                               : launch_shared_tc_as<false, false>(map, t, n_items, pdl, stream);
   }
 }
 

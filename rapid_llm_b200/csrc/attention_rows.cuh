@@ -12,6 +12,10 @@
 // an operand pair); P^T is S^T's fragment, transposed by movmatrix.  Sixteen 16-byte loads a lane fly per step (8 KB a
 // warp, some 100 KB a multiprocessor).
 //
+// Bound by the latency of those loads: 64 requests' 512 own keys (784 items, 128 MB) 21 us, 6.4 TB/s; 60 keys each 5 us.  Four
+// CTAs a multiprocessor (126 registers) instead of three 43 -> 40.5 us for the step with 8,192 shared keys; eight warps a CTA
+// were slower, and so were tiles by TMA into shared memory (23 -> 13.5 us for 16 requests of 2,048 shared keys).
+//
 // Scores, maxima, sums and O are float32; P is rounded to bfloat16 before P.V, as in attention_mma.cu.  Heads of 64 and 128,
 // pages of any size (a step inside one page, as with pages of 16 and its multiples, looks one page id up for the whole warp).
 #pragma once

@@ -1,8 +1,9 @@
 // Copies of cache pages: pages[layer, target] = pages[layer, source] for a list of (source, target) pairs, all layers of a
 // group in one launch.  What a fork needs for the page its branches go on writing in, what compaction moves.
 //
-// A pure stream: it reads and writes every byte once, so the copy rate bounds it.  The pairs ride in the launch's
-// parameters, so a call uploads nothing and waits for nothing, and a captured call keeps them.  The host has made sure
+// A pure stream: it reads and writes every byte once, so the copy rate bounds it: 600 pages of 64 KB in 36 layers take 427 us,
+// 6.6 TB/s; one page's seven copies in 36 layers 4.3 us, 19 MB, most of it the launch.  The pairs ride in the launch's parameters, so a
+// call uploads nothing and waits for nothing, and a captured call keeps them.  The host has made sure
 // that no page is written twice and none both read and written, so the order of the CTAs does not matter.  Rows of any size are
 // taken (per-request states are copied by the same kernel): the unit of a copy is the largest of 16, 8, 4, 2 and 1
 // bytes that a page is a multiple of and its address aligned to.
@@ -25,7 +26,7 @@ constexpr int kFewPairs = 60, kSomePairs = 500, kManyPairs = 3900;
 template <typename U, int kPairs>
 __global__ void __launch_bounds__(kCopyThreads)
 copy_pages_kernel(const __grid_constant__ PagePairs<kPairs> pairs, U* pages, long long layer_units, long long page_units) {
-  pdl_trigger();
+  // (No early start for what follows: attention may fetch cached keys before it waits, and these are some.)
   const int2 pair = pairs.of[blockIdx.y];
   U* layer = pages + static_cast<long long>(blockIdx.z) * layer_units;
   const U* src = layer + pair.x * page_units;

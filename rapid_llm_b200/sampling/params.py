@@ -43,11 +43,11 @@ class SamplingParams:
             raise ValueError(f"repetition_penalty must be > 0, got {self.repetition_penalty}")
         if self.logprobs is not None or self.prompt_logprobs is not None:
             raise ValueError("logprobs and prompt_logprobs are not reported by this engine; leave them None")
-        if self.top_k < 0 or self.top_k != int(self.top_k):
+        if self.top_k < 0 or self.top_k % 1 != 0:
             raise ValueError(f"top_k must be a whole number >= 0 (0 = all), got {self.top_k}")
         if not 0.0 <= self.min_p <= 1.0:
             raise ValueError(f"min_p must be in [0, 1], got {self.min_p}")
-        if self.n < 1 or self.n != int(self.n):
+        if self.n < 1 or self.n % 1 != 0:
             raise ValueError(f"n must be a whole number >= 1, got {self.n}")
         if self.seed is not None and not 0 <= self.seed < 2**63:
             raise ValueError(f"seed must be in [0, 2**63), got {self.seed}")

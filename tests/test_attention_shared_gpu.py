@@ -299,3 +299,41 @@ def test_a_nan_that_is_seen_stays_one(dtype, dim):
         step.cache[int(step.table[step.slots[0], 4]), 0, 1, 5] = float("nan")
         got = step.run().view(-1, 4, dim)
         assert bool(got[:members, 2:].isnan().all()) and torch.equal(got[members:], clean.view(-1, 4, dim)[members:])
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 128), (torch.bfloat16, 128), (torch.bfloat16, 64)])
+def test_pages_beyond_32_bits(dtype, dim):
+    """The same rows in pages whose first number lies behind 2^31 numbers and more: the same bits."""
+    step = Step([160, 37], [(0, 5 + 30 * i, 1) for i in range(9)] + [(1, 70, 2), (1, 3, 1)], heads=16, kv_heads=8, dim=dim, page=16, dtype=dtype)
+    near = step.run()
+    held = step.cache.shape[0]
+    first = 2**31 // step.cache[0].numel() + 5
+    cache = torch.zeros((first + held, *step.cache.shape[1:]), dtype=dtype, device=DEV)
+    cache[first:] = step.cache
+    step.cache, step.table = cache, np.where(step.table > 0, step.table + first, 0).astype(np.int32)
+    assert torch.equal(step.run(), near)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.bfloat16, 128), (torch.bfloat16, 64)])
+def test_calls_side_by_side(dtype, dim):
+    """Two steps on two streams, each with scratch and a result of its own."""
+    steps = [Step([2048], [(0, 1 + 40 * i, 1) for i in range(n)], heads=16, kv_heads=4, dim=dim, page=16, dtype=dtype, seed=n) for n in (12, 30)]
+    want = [step.run() for step in steps]
+    to = lambda values: torch.from_numpy(np.ascontiguousarray(np.asarray(values, dtype=np.int32))).to(DEV)
+    calls = []
+    for step in steps:
+        plan = step.device_plan()
+        rows = step.planner.part_rows(plan)
+        calls.append((step, torch.cuda.Stream(), torch.zeros_like(step.q), dict(
+            plan=plan, part_out=torch.empty((rows, dim), device=DEV), part_lse=torch.empty((rows,), device=DEV), positions=to(step.positions),
+            cu_seqlens=to(np.arange(len(step.new) + 1)), entry_start=to(step.starts), entry_slot=to(step.slots), block_table=to(step.table),
+            num_heads=16, num_kv_heads=4, head_dim=dim, scale=step.scale, fault=step.fault)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for step, stream, out, arguments in calls:
+            with torch.cuda.stream(stream):
+                out.fill_(float("nan"))
+                kernels.attention_shared(step.q, step.cache, out, **arguments)
+    torch.cuda.synchronize()
+    for (step, _, out, _), expected in zip(calls, want):
+        assert torch.equal(out, expected) and int(step.fault.item()) == 0

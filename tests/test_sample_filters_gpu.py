@@ -235,3 +235,39 @@ def test_refused(name, value):
     arguments[name] = value()
     with pytest.raises(kernels.KernelError):
         kernels.sample(arguments.pop("logits"), arguments.pop("out"), **arguments)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [1e-44, 3e-39, 3e38, float("inf")])
+def test_temperatures_at_the_ends_of_the_type(temperature):
+    for top_k, top_p, min_p in ((0, 1.0, 0.0), (30, 0.9, 0.0), (0, 0.7, 0.5), (2000, 0.9, 0.0)):
+        run_case(logits_of(6, 20011, torch.float32, seed=2), temperature, top_k, top_p, min_p, draws(6))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_the_largest_vocabulary(dtype):
+    largest = kernels.core().rl_sample_filtered_max_vocab()
+    for top_k, top_p in ((0, 0.9), (40, 0.9), (largest - 1, 0.99)):
+        run_case(logits_of(3, largest, dtype, seed=top_k), 1.0, top_k, top_p, 0.0, draws(3))
+    with pytest.raises(kernels.KernelError):
+        run_case(logits_of(3, largest + 1, dtype), 1.0, 40, 0.9, 0.0, draws(3))
+
+
+@pytest.mark.gpu
+def test_calls_side_by_side():
+    calls = []
+    for seed, (rows, vocab) in enumerate(((70, 32003), (9, 151936))):
+        x = logits_of(rows, vocab, torch.bfloat16, seed=seed)
+        of = lambda v, dtype=torch.float32: torch.full((rows,), v, dtype=dtype, device=DEV)
+        arguments = dict(temperature=of(0.9), top_k=of(0, torch.int32), top_p=of(0.95), uniforms=draws(rows, seed=seed).float().to(DEV))
+        calls.append((x, arguments, torch.cuda.Stream(), of(-7, torch.int32), kernels.sample(x, of(-7, torch.int32), **arguments)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for x, arguments, stream, out, _ in calls:
+            with torch.cuda.stream(stream):
+                out.fill_(-7)
+                kernels.sample(x, out, **arguments)
+    torch.cuda.synchronize()
+    for _, _, _, out, want in calls:
+        assert torch.equal(out, want)

@@ -113,7 +113,8 @@ def test_seeds():
     assert request.seed == 2**63 - 5 and all(0 <= r.seed < 2**63 for r in request.completions) and len({r.seed for r in request.completions}) == 4
 
 
-@pytest.mark.parametrize("wrong", [{"top_k": -1}, {"top_k": 1.5}, {"min_p": -0.1}, {"min_p": 1.1}, {"n": 0}, {"n": 2.5}])
+@pytest.mark.parametrize("wrong", [{"top_k": -1}, {"top_k": 1.5}, {"min_p": -0.1}, {"min_p": 1.1}, {"n": 0}, {"n": 2.5},
+                                   {"top_k": float("inf")}, {"n": float("inf")}, {"top_k": float("nan")}])
 def test_refused_parameters(wrong):
     with pytest.raises(ValueError):
         SamplingParams(**wrong)
