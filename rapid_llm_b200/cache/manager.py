@@ -333,7 +333,9 @@ class CacheManager:
         copied = [bool(ragged) and pages[whole] != NULL_PAGE for pages in held.pages]
         if any(copy and len(children) > pool.num_free for copy, pool in zip(copied, self.pools)):
             return None
-        if whole and held.family is None and children:
+        # (a family whose other members have gone is over: a new one shares all that is there by now)
+        alone = held.family is None or not any(other is not held and other.family == held.family for other in self._held.values())
+        if whole and alone and children:
             self._families += 1
             held.family = (self._families, whole * self.page_size)
         copies: list[list[tuple[int, int]]] = [[] for _ in self.groups]

@@ -180,3 +180,18 @@ def test_random_lives(seed):
                         assert (cache.block_tables[0][cache.slot_of(other), :count] == cache.block_tables[0][cache.slot_of(name), :count]).all()
                         assert cache.shared_prefix(other) == family and len(history[other]) >= family[1]
     assert isinstance(cache.block_tables[0], np.ndarray)
+
+
+def test_who_is_left_of_a_family_forks_anew():
+    cache = manager()
+    cache.admit("p")
+    assert cache.reserve("p", 9)
+    cache.fork("p", ["a", "b"])
+    assert cache.reserve("p", 21)
+    cache.release("a")
+    assert cache.fork("p", ["c"]) == [[(cache.pages_of("p")[0][5], cache.pages_of("c")[0][5])]]
+    assert cache.shared_prefix("c") == cache.shared_prefix("b") == cache.shared_prefix("p") and cache.shared_prefix("p")[1] == 8
+    cache.release("b"), cache.release("c")
+    cache.fork("p", ["d"])
+    assert cache.shared_prefix("d") == cache.shared_prefix("p") and cache.shared_prefix("d")[1] == 20
+    cache.check()
