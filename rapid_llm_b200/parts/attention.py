@@ -264,7 +264,7 @@ class SharedItems(StepPlanner):
     # Measured times in microseconds by the rows of a tile: an item's start (page ids, queries, first keys, result), a block of 128
     # keys (64 in the float32 tiles of 32 rows) of an item by itself, and how many items a multiprocessor runs at one time; the
     # block of a row item when its neighbours stream too; the join of the parts: its start, a part, a part of 1,024 rows.
-    COSTS = {256: (7.0, 1.85, 1), 128: (6.0, 0.95, 1), 64: (4.0, 6.0, 3), 32: (5.0, 4.0, 2), 16: (5.0, 0.9, 4)}
+    COSTS = {256: (7.0, 1.85, 1), 128: (6.0, 0.95, 1), 64: (4.0, 6.0, 3), 32: (5.0, 4.0, 2), 16: (5.0, 2.4, 4)}
     STREAMED_BLOCK = 1.5
     JOIN = (2.0, 0.05, 0.35)
     STEPS = np.array([1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64, 96, 128, 192, 256, 512, 1024, 4096, 1 << 20])
