@@ -12,9 +12,12 @@
 // an operand pair); P^T is S^T's fragment, transposed by movmatrix.  Sixteen 16-byte loads a lane fly per step (8 KB a
 // warp, some 100 KB a multiprocessor).
 //
-// Bound by the latency of those loads: 64 requests' 512 own keys (784 items, 128 MB) 21 us, 6.4 TB/s; 60 keys each 5 us.  Four
-// CTAs a multiprocessor (126 registers) instead of three 43 -> 40.5 us for the step with 8,192 shared keys; eight warps a CTA
-// were slower, and so were tiles by TMA into shared memory (23 -> 13.5 us for 16 requests of 2,048 shared keys).
+// By themselves, with the join: 64 requests of 8 key heads and 512 keys 27.8 us for 20.5 of HBM's rate, 2,048 keys 90 for 82,
+// 16 keys 6.6; heads of 64 (4 key heads) 2,048 keys 47 for 20.5: half the bytes in flight, so the loads' latency bounds them.
+// An item by itself takes 1.3 us a step of its warps.  Four CTAs a multiprocessor (126 registers) instead of three 43 ->
+// 40.5 us for 64 requests behind 8,192 shared keys; eight warps a CTA were slower, so were tiles by TMA into shared memory
+// (13.5 -> 23 us for 16 requests behind 2,048) and the next step's keys ahead, for which the queries had to leave the
+// registers (27.8 -> 35.9 us for the 512 keys, heads of 64 16.2 -> 16.8).
 //
 // Scores, maxima, sums and O are float32; P is rounded to bfloat16 before P.V, as in attention_mma.cu.  Heads of 64 and 128,
 // pages of any size (a step inside one page, as with pages of 16 and its multiples, looks one page id up for the whole warp).

@@ -263,7 +263,8 @@ class SharedItems(StepPlanner):
 
     # Measured times in microseconds by the rows of a tile: an item's start (page ids, queries, first keys, result), a block of 128
     # keys (64 in the float32 tiles of 32 rows) of an item by itself, and how many items a multiprocessor runs at one time; the
-    # block of a row item when its neighbours stream too; the join of the parts: its start, a part, a part of 1,024 rows.
+    # block of a row item when its neighbours stream too; the join of the parts: its start, a part, a part of 1,024 rows.  (A row item's
+    # block by itself taken as 0.9 us, a CTA's share of the rate: 8 requests of 4,096 + 300 keys 16.9 instead of 12.2 us.)
     COSTS = {256: (7.0, 1.85, 1), 128: (6.0, 0.95, 1), 64: (4.0, 6.0, 3), 32: (5.0, 4.0, 2), 16: (5.0, 2.4, 4)}
     STREAMED_BLOCK = 1.5
     JOIN = (2.0, 0.05, 0.35)
@@ -404,10 +405,10 @@ class SharedItems(StepPlanner):
 
 # Bytes of keys and values, read again by every member but one of groups with so many members, from which on a decode step reads
 # shared prefixes once.  Measured with 8 key heads of 128 and groups of 4 in bfloat16, us in a captured step, ordinary against shared,
-# at requests x shared positions: 2 x 1,024 8.0 and 7.9, 2 x 16,384 (67 MB) 23.4 and 26.9, 4 x 1,024 (13 MB) 9.4 and 9.6, 4 x 4,096
-# (50 MB) 14.1 and 14.5, 8 x 256 (7 MB) 8.7 and 7.9, 8 x 1,024 (29 MB) 10.8 and 9.0, 8 x 4,096 20.2 and 15.8, 8 x 16,384 62 and 20,
-# 16 x 512 (31 MB) 8.8 and 8.5, 16 x 2,048 17.8 and 10.6, 32 x 512 (65 MB) 12.3 and 10.4, 64 x 256 (66 MB) 18.9 and 13.3, 64 x 1,024 36 and 18,
-# 64 x 8,192 220 and 40.
+# at requests x shared positions: 2 x 1,024 8.1 and 7.9, 2 x 16,384 (67 MB) 23.4 and 26.9, 4 x 1,024 (13 MB) 9.4 and 9.7, 4 x 4,096
+# (50 MB) 14.1 and 14.9, 8 x 256 (7 MB) 8.7 and 8.0, 8 x 1,024 (29 MB) 10.9 and 9.2, 8 x 4,096 20.2 and 14.2, 8 x 16,384 62 and 20,
+# 16 x 512 (31 MB) 8.7 and 8.5, 16 x 2,048 17.9 and 10.4, 32 x 512 (65 MB) 12.3 and 10.4, 64 x 256 (66 MB) 18.8 and 13.1, 64 x 1,024 36 and 18,
+# 64 x 8,192 220 and 41.
 WORTH_SHARING = 12 << 20
 MEMBERS_WORTH_SHARING = 5
 # ... and in float32, where the other kernel gives every row a warp of its own: 8 heads in groups of 4, 2 x 64 (0.02 MB) 22 and 8 us,
