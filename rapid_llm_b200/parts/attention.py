@@ -256,16 +256,19 @@ class SharedItems(StepPlanner):
         self.wide = dtype == torch.float32
         self.tag = kernels.dtype_tag(dtype)
         self.key = ("shared_items", self.group, self.num_kv_heads, self.head_dim, self.sms, self.tag)
+        # The float32 tiles' products and shared memory grow with the head: two of them fit a multiprocessor up to 144 numbers.  (3 requests
+        # with 15,568 shared keys of 256: 87 us as one a multiprocessor, 130 as two; 8 with 4,096 of 64: 21 us at half the cost, 27 at all of it.)
+        self.costs = {**self.COSTS, 32: (5.0, 4.0 * self.head_dim / 128, 2 if self.head_dim <= 144 else 1)}
 
     def part_rows(self, plan: dict) -> int:
         """Rows of the two scratch buffers."""
         return plan["parts"] * self.group * self.num_kv_heads
 
     # Measured times in microseconds by the rows of a tile: an item's start (page ids, queries, first keys, result), a block of 128
-    # keys (64 in the float32 tiles of 32 rows) of an item by itself, and how many items a multiprocessor runs at one time; the
+    # keys (64 in the float32 tiles of 32 rows, whose times depend on the head) of an item by itself, and how many items a multiprocessor runs at one time; the
     # block of a row item when its neighbours stream too; the join of the parts: its start, a part, a part of 1,024 rows.  (A row item's
     # block by itself taken as 0.9 us, a CTA's share of the rate: 8 requests of 4,096 + 300 keys 16.9 instead of 12.2 us.)
-    COSTS = {256: (7.0, 1.85, 1), 128: (6.0, 0.95, 1), 64: (4.0, 6.0, 3), 32: (5.0, 4.0, 2), 16: (5.0, 2.4, 4)}
+    COSTS = {256: (7.0, 1.85, 1), 128: (6.0, 0.95, 1), 64: (4.0, 6.0, 3), 16: (5.0, 2.4, 4)}
     STREAMED_BLOCK = 1.5
     JOIN = (2.0, 0.05, 0.35)
     STEPS = np.array([1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64, 96, 128, 192, 256, 512, 1024, 4096, 1 << 20])
@@ -285,12 +288,12 @@ class SharedItems(StepPlanner):
             end = start + block * np.minimum(steps[:, None], blocks[None]).max(1)
             return steps, (ranges * side).sum(1), end, ranges.max(1), together, int((blocks * side).sum())
 
-        tile_steps, tile_items, tile_end, tile_parts, tile_together, _ = of(tiles, self.COSTS[tile_rows])
-        row_steps, row_items, row_end, row_parts, row_together, row_blocks = of(rows, self.COSTS[kernels.DECODE_TILE_ROWS])
+        tile_steps, tile_items, tile_end, tile_parts, tile_together, _ = of(tiles, self.costs[tile_rows])
+        row_steps, row_items, row_end, row_parts, row_together, row_blocks = of(rows, self.costs[kernels.DECODE_TILE_ROWS])
         tile_items, tile_end, tile_parts = tile_items[:, None], tile_end[:, None], tile_parts[:, None]
         tiles_done = np.ceil(tile_items / (self.sms * tile_together)) * tile_end
         left = np.maximum(self.sms - tile_items / tile_together, 0)
-        row_work = row_items * (self.COSTS[kernels.DECODE_TILE_ROWS][0] / row_together) + row_blocks * self.STREAMED_BLOCK
+        row_work = row_items * (self.costs[kernels.DECODE_TILE_ROWS][0] / row_together) + row_blocks * self.STREAMED_BLOCK
         # the last items' share of the time behind: streaming beside three others, a block takes as many times as long
         longest = np.minimum(row_steps, int(np.asarray(rows)[:, 0].max())) if len(rows) else np.zeros(1)
         behind = np.maximum(row_work - 0.8 * left * tiles_done, 0) / self.sms + 0.25 * (5.0 + self.STREAMED_BLOCK * row_together * longest)
