@@ -337,3 +337,12 @@ def test_calls_side_by_side(dtype, dim):
     torch.cuda.synchronize()
     for (step, _, out, _), expected in zip(calls, want):
         assert torch.equal(out, expected) and int(step.fault.item()) == 0
+
+
+@pytest.mark.parametrize("page", [16, 20])
+@pytest.mark.parametrize("dim", [16, 32, 80, 144, 256])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_every_head_size(dtype, dim, page):
+    step = Step([400, 90], [(0, 1 + 37 * i, 1) for i in range(7)] + [(1, 250, 2), (1, 3, 1), (-1, 130, 3)], heads=6, kv_heads=2, dim=dim,
+                page=page, dtype=dtype, seed=dim)
+    check(step.run(), step.want(), dtype, dim)
