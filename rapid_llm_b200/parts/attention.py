@@ -407,12 +407,14 @@ class SharedItems(StepPlanner):
 
 
 # Bytes of keys and values, read again by every member but one of groups with so many members, from which on a decode step reads
-# shared prefixes once.  Measured with 8 key heads of 128 and groups of 4 in bfloat16, us in a captured step, ordinary against shared,
-# at requests x shared positions: 2 x 1,024 8.1 and 7.9, 2 x 16,384 (67 MB) 23.4 and 26.9, 4 x 1,024 (13 MB) 9.4 and 9.7, 4 x 4,096
-# (50 MB) 14.1 and 14.9, 8 x 256 (7 MB) 8.7 and 8.0, 8 x 1,024 (29 MB) 10.9 and 9.2, 8 x 4,096 20.2 and 14.2, 8 x 16,384 62 and 20,
-# 16 x 512 (31 MB) 8.7 and 8.5, 16 x 2,048 17.9 and 10.4, 32 x 512 (65 MB) 12.3 and 10.4, 64 x 256 (66 MB) 18.8 and 13.1, 64 x 1,024 36 and 18,
-# 64 x 8,192 220 and 41.
-WORTH_SHARING = 12 << 20
+# shared prefixes once.  Measured in whole steps, where an ordinary layer's one kernel starts under the kernels before it and a sharing
+# layer's three follow one another: 36 layers of 8 key heads of 128 in groups of 4, bfloat16, ms a captured step, ordinary against
+# shared, at requests x shared positions (MB a layer): 2 x 16,384 (67) 3.71 and 4.38, 4 x 4,096 (50) 3.38 and 3.50, 4 x 16,384 (201) 4.02
+# and 3.98, 8 x 1,024 (29) 3.30 and 3.37, 8 x 2,048 (59) 3.40 and 3.43, 12 x 2,048 (92) 3.57 and 3.63, 8 x 4,096 (117) 3.62 and 3.48,
+# 8 x 16,384 5.13 and 3.75, 16 x 512 (31) 3.30 and 3.48, 16 x 2,048 (126) 3.64 and 3.56, 32 x 512 (65) 3.67 and 3.80, 32 x 1,024 (130) 3.87 and
+# 3.88, 32 x 4,096 5.09 and 3.96, 64 x 256 (66) 4.25 and 4.16, 64 x 512 (132) 4.46 and 4.41, 64 x 1,024 4.86 and 4.47, 64 x 8,192 11.1 and
+# 4.9.  By themselves on an idle GPU the kernels would already pay from 12 MB on (8 x 4,096 20.2 and 14.2 us, 64 x 8,192 220 and 41).
+WORTH_SHARING = 96 << 20
 MEMBERS_WORTH_SHARING = 5
 # ... and in float32, where the other kernel gives every row a warp of its own: 8 heads in groups of 4, 2 x 64 (0.02 MB) 22 and 8 us,
 # 8 x 128 39 and 11, 8 x 2,048 566 and 13.
