@@ -289,7 +289,10 @@ struct Row {
         if (kMass) m += static_cast<double>(ranks == 1 ? s.mass[buffer][b] : peer_u32(&s.mass[buffer][b], r));
       }
       s.counts[b] = kCount ? n : m > 0.0;
-      if (kMass) s.total[b] = m * (1.0 / 32768.0) * exp2(-static_cast<double>(at.low + (static_cast<unsigned>(b) << shift)) * back * (per * (1.0 / 64.0)));
+      if (kMass) {
+        const double edge = static_cast<double>(at.low + (static_cast<unsigned>(b) << shift)) * back;
+        s.total[b] = m * (1.0 / 32768.0) * exp2(-edge * (per * (1.0 / 64.0)));
+      }
     }
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -439,7 +442,9 @@ constexpr int kRoomyBytes = 96 * 1024;        // of a slice of which two fit a m
 
 static int sm_count() {
   int device = 0, sms = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 148;
+  if (cudaGetDevice(&device) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0)
+    sms = 148;
   return sms;
 }
 
@@ -742,11 +747,10 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       z = sums[0];
       above = sums[1];
       inside = sums[2];
-      const unsigned front_n = static_cast<unsigned>(sums[3] >> 32);
       behind = sums[3] & 0xffffffffull;
       const double budget = fmax(static_cast<double>(p), 0.0) * static_cast<double>(z);
       if (static_cast<double>(above) > budget) {       // (not met: the approximate masses are nearer than their slack)
-        at = {0u, at.low - 1u, 0u, front_n, 0.0};
+        at = {0u, at.low - 1u, 0u, static_cast<unsigned>(sums[3] >> 32), 0.0};
         above = 0;
         weighed = 0;
         weighed_to = 0;
