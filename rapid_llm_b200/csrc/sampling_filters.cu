@@ -605,8 +605,31 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       }
       if (fewer || at.above_n + at.inside_n <= kList || at.low == at.high || (at.inside_n <= kList && want_k > kList)) break;
     }
+    // The k-th value, whose place among the ordered ones is in a .. b, and the index of its last one that stays.
+    auto bisect = [&](unsigned a, unsigned b) {
+      while (a < b) {
+        const unsigned mid = a + (b - a) / 2;
+        u64 n = 0;
+        row.sweep_any([&](int, float v) { n += ordered(v) > mid; });
+        if (row.cluster_sum(n) >= static_cast<u64>(want_k)) a = mid + 1; else b = mid;
+      }
+      cut_k = unordered(a);
+      u64 n = 0;
+      row.sweep_any([&](int, float v) { n += ordered(v) > a; });
+      const u64 ties = static_cast<u64>(want_k) - row.cluster_sum(n);    // of the equal ones so many stay
+      int from = 0, to = args.vocab - 1;
+      while (from < to) {
+        const int mid = from + (to - from) / 2;
+        n = 0;
+        row.sweep_any([&](int i, float v) { n += ordered(v) == a && row.begin + i <= mid; });
+        if (row.cluster_sum(n) >= ties) to = mid; else from = mid + 1;
+      }
+      cut_i = from;
+    };
     if (fewer) {
-      // nothing is cut
+      // Nothing is cut, as what lies beyond the codes weighs nothing.  But u = 0 may take a token out there, so the cut is
+      // looked for by values, over the whole row.
+      if (first_of_all) bisect(ordered(-INFINITY), ordered(top));
     } else if (at.above_n + at.inside_n <= kList) {
       // the whole of top-k and a little more fits the list: everything else happens there
       const unsigned n = row.template gather<true>(0u, at.high, everything);
@@ -671,25 +694,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
       // more tokens than the list holds within one code: bisect their values, then their indices
       float high, low;
       row.range_of(at, everything, high, low);
-      unsigned a = ordered(low), b = ordered(high);           // the k-th value lies in a .. b
-      while (a < b) {
-        const unsigned mid = a + (b - a) / 2;
-        u64 n = 0;
-        row.sweep_any([&](int, float v) { n += ordered(v) > mid; });
-        if (row.cluster_sum(n) >= static_cast<u64>(want_k)) a = mid + 1; else b = mid;
-      }
-      cut_k = unordered(a);
-      u64 n = 0;
-      row.sweep_any([&](int, float v) { n += ordered(v) > a; });
-      const u64 ties = static_cast<u64>(want_k) - row.cluster_sum(n);    // of the equal ones so many stay
-      int from = 0, to = args.vocab - 1;
-      while (from < to) {
-        const int mid = from + (to - from) / 2;
-        n = 0;
-        row.sweep_any([&](int i, float v) { n += ordered(v) == a && row.begin + i <= mid; });
-        if (row.cluster_sum(n) >= ties) to = mid; else from = mid + 1;
-      }
-      cut_i = from;
+      bisect(ordered(low), ordered(high));
     }
   }
   auto in_k = [&](int i, float v) { return v > cut_k || (v == cut_k && row.begin + i <= cut_i); };
