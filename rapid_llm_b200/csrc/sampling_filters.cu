@@ -582,8 +582,11 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   }
   const bool by_rank = want_k > 0 && want_k < args.vocab, by_mass = p < 1.0f;
   const bool first_of_all = !(u > 0.0f);
-  // whether the weight is more than zero in float64
-  auto counts_at_all = [&](float v) { return exp((static_cast<double>(v) - static_cast<double>(top)) / static_cast<double>(temp)) > 0.0; };
+  // whether min-p leaves a weight, which may be too small for the whole multiples: in float64, and more than zero there
+  auto left_at_zero = [&](float v) {
+    const double w = exp((static_cast<double>(v) - static_cast<double>(top)) / static_cast<double>(temp));
+    return w > 0.0 && w >= static_cast<double>(least_p);
+  };
   auto target_of = [&](u64 mass) {
     const double t = u > 0.0f ? static_cast<double>(u) * static_cast<double>(mass) : 0.0;
     return t >= static_cast<double>(mass) ? mass - 1 : min(static_cast<u64>(t), mass - 1);
@@ -661,7 +664,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
         keep = keep && (static_cast<double>(above) <= static_cast<double>(p) * static_cast<double>(z) || my_x == top);
         __syncthreads();
       }
-      keep = keep && (static_cast<double>(my_w) >= least_weight) && (my_w > 0 || (first_of_all && counts_at_all(my_x)));
+      keep = keep && (first_of_all ? left_at_zero(my_x) : my_w > 0 && static_cast<double>(my_w) >= least_weight);
       if (lead && have) s.all_keep[mine] = keep;
       const u64 mass = row.block_sum(lead && keep ? my_w : 0ull);
       u64 before = 0;
@@ -822,7 +825,7 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   if (first_of_all) {
     unsigned best = 0;                               // the complement of the first index
     row.sweep([&](int i, float v) {
-      if (best == 0 && v > -INFINITY && v >= cut_p && in_k(i, v) && counts_at_all(v) && static_cast<double>(row.weight(v)) >= least_weight)
+      if (best == 0 && v > -INFINITY && v >= cut_p && in_k(i, v) && left_at_zero(v))
         best = ~static_cast<unsigned>(row.begin + i);
     });
     u64 one[1] = {best};
