@@ -384,8 +384,8 @@ class SharedItems(StepPlanner):
 
     def step_plan(self, shape: StepShape) -> dict | None:
         """The plan of a decode-only step where sharing is worth its launches, else ``None``.  The lists are filled up with empty
-        items and the number of parts is rounded up, to powers of two: what a captured step has baked in then changes at few
-        context lengths."""
+        items and the number of parts is rounded up, to powers of two, and the members' list has one size for all steps of a batch size:
+        what a captured step has baked in then changes at few context lengths and not as members of a group end."""
         if not shape.decode_only or shape.prefix_group is None:
             return None
         saved = self.saved_bytes(shape)
@@ -398,6 +398,9 @@ class SharedItems(StepPlanner):
             padded = np.zeros((up(len(items)), kernels.SHARED_ITEM), dtype=np.int32)
             padded[: len(items)] = items
             plan[name] = padded
+        members = np.zeros(2 * plan["tokens"], dtype=np.int32)         # a token is listed for its entry and in one group at most
+        members[: len(plan["members"])] = plan["members"]
+        plan["members"] = members
         if 8 * (len(plan["tile_items"]) + len(plan["row_items"])) > self.capacity(len(shape.lengths), len(shape.lengths)) - 3 * len(shape.lengths) - 64:
             return None
         return {**plan, "parts": up(plan["parts"]), "shared": True}
