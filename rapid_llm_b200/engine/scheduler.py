@@ -226,12 +226,12 @@ class Scheduler:
             request_id = f"req-{next(self._ids)}"
         seed = params.seed if params.seed is not None else zlib.crc32(repr(request_id).encode())
         request = Request(request_id, prompt, params, max_new, seed, arrival_time=time.perf_counter())
-        self.waiting.append(request)
         others = [
             Request((request_id, index), prompt, params, max_new, (seed + index * SEED_STRIDE) % 2**63, arrival_time=request.arrival_time)
             for index in range(1, params.n)
         ]
         request.completions = [request, *others]
+        self.waiting.append(request)
         if others and len(prompt) > 1 and hasattr(self.executor, "fork"):
             self._to_fork[request_id] = others
         else:

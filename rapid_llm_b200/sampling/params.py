@@ -49,6 +49,7 @@ class SamplingParams:
             raise ValueError(f"min_p must be in [0, 1], got {self.min_p}")
         if self.n < 1 or self.n % 1 != 0:
             raise ValueError(f"n must be a whole number >= 1, got {self.n}")
+        self.top_k, self.n = int(self.top_k), int(self.n)      # (2.0 is a whole number too)
         if self.seed is not None and not 0 <= self.seed < 2**63:
             raise ValueError(f"seed must be in [0, 2**63), got {self.seed}")
 

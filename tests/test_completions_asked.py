@@ -1,0 +1,29 @@
+"""How many completions a request asks for, in whatever number type, and what a refused request leaves behind."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+from test_scheduler_completions import scheduler_of, several
+
+from rapid_llm_b200.sampling import SamplingParams
+
+
+@pytest.mark.parametrize("n", [2, 2.0, np.int64(2), np.float32(2)])
+def test_whole_numbers_of_any_type(n):
+    params = several(n, 3, top_k=5.0)
+    assert type(params.n) is int and type(params.top_k) is int and (params.n, params.top_k) == (2, 5)
+    scheduler, executor = scheduler_of()
+    request = scheduler.add_request(list(range(20)), params, "a")
+    scheduler.run_to_completion()
+    assert [len(r.output_token_ids) for r in request.completions] == [3, 3]
+    assert executor.cache.num_free_slots == 4
+
+
+def test_a_request_that_fails_leaves_nothing_in_the_queue():
+    params = SamplingParams(temperature=0.0, repetition_penalty=1.0, max_gen_len=3)
+    params.n = 2.5                                    # changed after it was checked
+    scheduler, _ = scheduler_of()
+    with pytest.raises(TypeError):
+        scheduler.add_request(list(range(20)), params, "a")
+    assert not scheduler.waiting and not scheduler.has_unfinished()
