@@ -25,8 +25,8 @@ with ``stop_on_repeat`` is checked for a loop (``engine/repetition.py``), as the
 
 Several completions of one prompt (``SamplingParams.n``): the first of them computes the prompt, its last token left out;
 there the others are forked from it (they share its pages, see ``CacheManager.fork``), and all of them feed that token side by
-side and sample on their own.  Those that find no slot or page then, and those whose prompt has one token, compute the
-prompt themselves, like requests of their own.
+side and sample on their own.  If it is aborted before that, the next of them takes its part.  Those that find no slot or
+page at the fork, and those whose prompt has one token, compute the prompt themselves, like requests of their own.
 
 Running ahead.  A step's sampled tokens stay on the device, where the next step's embedding
 can pick them up, so the next step can be planned and enqueued before the host has seen them:
@@ -458,7 +458,10 @@ class Scheduler:
             for others in self._to_fork.values():        # not forked yet
                 if request in others:
                     others.remove(request)
-        self.waiting.extendleft(reversed(self._to_fork.pop(request.request_id, [])))      # no one computes their prompt any more
+        others = self._to_fork.pop(request.request_id, [])
+        if others:                                       # the next of them computes the prompt for those behind it
+            self.waiting.appendleft(others[0])
+            self._to_fork[others[0].request_id] = others[1:]
         self._to_fork = {leader: others for leader, others in self._to_fork.items() if others}
 
     def abort(self, request: Request | Hashable) -> None:
