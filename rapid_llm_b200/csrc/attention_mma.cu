@@ -979,8 +979,9 @@ int rl_attention_shared(const void* q, const void* cache, void* out, float* part
       n_tile_items > 65535 || n_row_items > 65535 || (tile_rows != 64 && tile_rows != 128 && tile_rows != 256) ||
       (tile_rows != 64 && !attn::decode_tc_supported(page_size)) ||
       static_cast<long long>(num_pages) * 2 * hkv * page_size > 0x7fffffffll || out_stride < hq * head_dim || out_stride % 8 != 0 ||
-      (reinterpret_cast<uintptr_t>(out) & 15) || (gate != nullptr && gate_stride < hq) ||
-      static_cast<long long>(tokens) * hq > 0x7fffffffll || parts < 0 || parts * hq > 0x7fffffffll)
+      ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) |
+        reinterpret_cast<uintptr_t>(part_out)) & 15) ||                      // all four are read or written 16 bytes at a time
+      (gate != nullptr && gate_stride < hq) || static_cast<long long>(tokens) * hq > 0x7fffffffll || parts < 0 || parts * hq > 0x7fffffffll)
     return static_cast<int>(cudaErrorInvalidValue);
   attn::AttentionArgs args = {};
   args.q = static_cast<const attn::bf16*>(q);

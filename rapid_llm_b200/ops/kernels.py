@@ -896,6 +896,8 @@ def attention_shared(
     if part_out is None or part_lse is None or part_out.numel() < parts * num_heads * head_dim or part_lse.numel() < parts * num_heads:
         raise KernelError("attention: scratch for the parts is missing or too small")
     scratch = _need_list("part_out", part_out, torch.float32, here), _need_list("part_lse", part_lse, torch.float32, here)
+    if (q_at | cache_at | scratch[0]) % 16:
+        raise KernelError("attention: q, cache and part_out must be 16-byte aligned")
     positions_at, slot_at, table_at, fault_at, tiles_at, rows_at, members_at, first_at, _, _ = at
     tiles, rows = plan["tile_items"].shape[0], plan["row_items"].shape[0]
     what = (tokens, num_heads, num_kv_heads, head_dim, shape[3], shape[0], block_table.shape[1], block_table.shape[0], float(scale),
