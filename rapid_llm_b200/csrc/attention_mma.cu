@@ -975,7 +975,7 @@ int rl_attention_shared(const void* q, const void* cache, void* out, float* part
                         int max_pages, int slots, float scale, const float* sink, const float* slopes, int out_stride,
                         const void* gate, int gate_stride, int* fault, int pdl, cudaStream_t stream) {
   if (tokens == 0) return 0;
-  if (head_dim != attn::kD || hkv <= 0 || hq % hkv != 0 || page_size <= 0 || hkv > 65535 || n_tile_items < 0 || n_row_items < 0 ||
+  if (head_dim != attn::kD || hkv <= 0 || hq % hkv != 0 || page_size <= 0 || num_pages <= 0 || hkv > 65535 || n_tile_items < 0 || n_row_items < 0 ||
       n_tile_items > 65535 || n_row_items > 65535 || (tile_rows != 64 && tile_rows != 128 && tile_rows != 256) ||
       (tile_rows != 64 && !attn::decode_tc_supported(page_size)) ||
       static_cast<long long>(num_pages) * 2 * hkv * page_size > 0x7fffffffll || out_stride < hq * head_dim || out_stride % 8 != 0 ||

@@ -271,7 +271,7 @@ int rl_attention_shared_f32(const float* q, const float* cache, float* out, floa
                             int max_pages, int slots, float scale, const float* sink, const float* slopes, int out_stride,
                             const float* gate, int gate_stride, int* fault, int pdl, cudaStream_t stream) {
   if (tokens == 0) return 0;
-  if (d <= 0 || d % 16 != 0 || d > 256 || hkv <= 0 || hq % hkv != 0 || page_size <= 0 || n_items < 0 || n_items > 65535 ||
+  if (d <= 0 || d % 16 != 0 || d > 256 || hkv <= 0 || hq % hkv != 0 || page_size <= 0 || num_pages <= 0 || n_items < 0 || n_items > 65535 ||
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(part_out)) & 15) ||
       out_stride < hq * d || (gate != nullptr && gate_stride < hq) || static_cast<long long>(tokens) * hq > 0x7fffffffll)
     return static_cast<int>(cudaErrorInvalidValue);

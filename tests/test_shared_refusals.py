@@ -26,3 +26,9 @@ KINDS = [("f32", 64, 64), ("bf16", 64, 64), ("bf16", 128, 128), ("bf16", 128, 25
 @pytest.mark.parametrize("name,off", [("q", 2), ("q", 4), ("q", 8), ("cache", 4), ("cache", 8), ("part_out", 4), ("part_out", 8)])
 def test_operands_that_are_read_sixteen_bytes_at_a_time(dtype, dim, tile_rows, name, off):
     assert call(dtype, dim, tile_rows, **{name: off}) == INVALID
+
+
+@pytest.mark.parametrize("dtype,dim,tile_rows", KINDS)
+def test_a_cache_without_pages(dtype, dim, tile_rows):
+    """A bad page id reads page 0 in its place, so there has to be one."""
+    assert call(dtype, dim, tile_rows, num_pages=0) == INVALID
