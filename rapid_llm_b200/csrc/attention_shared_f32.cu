@@ -59,6 +59,8 @@ attention_shared_f32_kernel(const SharedF32Args args) {
   __shared__ long long places[2][kSfKeys];               // where a block's key rows start (-1: beyond the end), alternating
   __shared__ int row_token[kSfRows], row_pos[kSfRows];
   __shared__ float row_slope[kSfRows];
+  __shared__ int first_pos;                              // the smallest of the rows' positions
+  static_assert(kSfRows == 32, "a row a lane of the first warp");
   constexpr int p_stride = kSfRows + kSfPad;
 
   pdl_trigger();
@@ -82,6 +84,8 @@ attention_shared_f32_kernel(const SharedF32Args args) {
     row_slope[r] = valid && args.slopes != nullptr ? args.slopes[head] * 1.4426950408889634f : 0.0f;
     row_max[r] = -INFINITY;
     row_sum[r] = 0.0f;
+    const int smallest = __reduce_min_sync(0xffffffffu, valid ? row_pos[r] : 0x7fffffff);      // (one warp, a row a lane)
+    if (r == 0) first_pos = smallest;
   }
   // a block's page ids are looked up once, by a thread a key, a block ahead of its copies
   const size_t head_elements = static_cast<size_t>(args.page_size) * d;
@@ -220,9 +224,12 @@ attention_shared_f32_kernel(const SharedF32Args args) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[u][i][e] *= alpha;
       }
-      const int last = min(kSfKeys, end - kb);
+      // Keys that all rows see; behind them, where tokens of one request differ, a row leaves out what it does not see:
+      // zero times a value that is not finite is no zero.
+      const int last = min(kSfKeys, end - kb), seen_by_all = min(last, first_pos - kb + 1);
+      int k = 0;
 #pragma unroll 4
-      for (int k = 0; k < last; ++k) {
+      for (; k < seen_by_all; ++k) {
         const float4 v = *reinterpret_cast<const float4*>(v_tile + k * stride + c);
         const float4 p = *reinterpret_cast<const float4*>(p_tile + k * p_stride + r0);
         const float w[4] = {p.x, p.y, p.z, p.w};
@@ -232,6 +239,19 @@ attention_shared_f32_kernel(const SharedF32Args args) {
           acc[u][i][1] = fmaf(w[i], v.y, acc[u][i][1]);
           acc[u][i][2] = fmaf(w[i], v.z, acc[u][i][2]);
           acc[u][i][3] = fmaf(w[i], v.w, acc[u][i][3]);
+        }
+      }
+#pragma unroll 1
+      for (; k < last; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(v_tile + k * stride + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (kb + k > row_pos[r0 + i]) continue;
+          const float w = p_tile[k * p_stride + r0 + i];
+          acc[u][i][0] = fmaf(w, v.x, acc[u][i][0]);
+          acc[u][i][1] = fmaf(w, v.y, acc[u][i][1]);
+          acc[u][i][2] = fmaf(w, v.z, acc[u][i][2]);
+          acc[u][i][3] = fmaf(w, v.w, acc[u][i][3]);
         }
       }
     }

@@ -870,7 +870,9 @@ def attention_shared(
     how many positions, and the block tables of a group's entries must name the same pages there.  ``part_out``
     ``[part_rows, head_dim]`` and ``part_lse`` ``[part_rows]`` (float32) are scratch of ``SharedItems.part_rows(plan)`` rows
     and more; calls that may run at the same time need scratch of their own.  ``sink``, ``gate`` and ``slopes`` as in :func:`attention_mma`, rows of ``out`` and
-    ``gate`` too; every key up to a token's own position is seen (no window, no squashed scores, caches of two planes)."""
+    ``gate`` too; every key up to a token's own position is seen (no window, no squashed scores, caches of two planes).  Where a request has
+    several new tokens, a value of a later one that is not finite leaves the earlier ones alone in float32; in bfloat16 it can reach
+    those in its tile as NaN, as in :func:`attention_mma` (zero times it, in the tensor cores)."""
     here, dtype = _here(q), q.dtype
     q_at, cache_at = _need_list("q", q, dtype, here), _need_list("cache", cache, dtype, here)
     at = [_need_list(name, tensor, torch.int32, here) for name, tensor in (
