@@ -388,8 +388,10 @@ class SharedItems(StepPlanner):
         what a captured step has baked in then changes at few context lengths and not as members of a group end."""
         if not shape.decode_only or shape.prefix_group is None:
             return None
-        saved = self.saved_bytes(shape)
-        if saved == 0 or saved < (WORTH_SHARING_F32 if self.wide else WORTH_SHARING):
+        saved, worth = self.saved_bytes(shape), WORTH_SHARING_F32 if self.wide else WORTH_SHARING
+        if np.count_nonzero(np.asarray(shape.prefix_group) >= 0) > FEW_SHARING:
+            worth += worth // 2
+        if saved == 0 or saved < worth:
             return None
         plan = self.plan(shape)
         up = lambda n: 0 if n == 0 else 1 << (int(n) - 1).bit_length()
@@ -410,14 +412,19 @@ class SharedItems(StepPlanner):
 
 
 # Bytes of keys and values, read again by every member but one of groups with so many members, from which on a decode step reads
-# shared prefixes once.  Measured in whole steps, where an ordinary layer's one kernel starts under the kernels before it and a sharing
-# layer's three follow one another: 36 layers of 8 key heads of 128 in groups of 4, bfloat16, ms a captured step, ordinary against
-# shared, at requests x shared positions (MB a layer): 2 x 16,384 (67) 3.71 and 4.38, 4 x 4,096 (50) 3.38 and 3.50, 4 x 16,384 (201) 4.02
-# and 3.98, 8 x 1,024 (29) 3.30 and 3.37, 8 x 2,048 (59) 3.40 and 3.43, 12 x 2,048 (92) 3.57 and 3.63, 8 x 4,096 (117) 3.62 and 3.48,
-# 8 x 16,384 5.13 and 3.75, 16 x 512 (31) 3.30 and 3.48, 16 x 2,048 (126) 3.64 and 3.56, 32 x 512 (65) 3.67 and 3.80, 32 x 1,024 (130) 3.87 and
-# 3.88, 32 x 4,096 5.09 and 3.96, 64 x 256 (66) 4.25 and 4.16, 64 x 512 (132) 4.46 and 4.41, 64 x 1,024 4.86 and 4.47, 64 x 8,192 11.1 and
-# 4.9.  By themselves on an idle GPU the kernels would already pay from 12 MB on (8 x 4,096 20.2 and 14.2 us, 64 x 8,192 220 and 41).
-WORTH_SHARING = 96 << 20
+# shared prefixes once; half as much again where more than FEW_SHARING requests share, whose shorter prefixes the ordinary kernel
+# reads again from L2.  Measured in whole steps of 36 layers of 8 key heads of 128 in groups of 4, bfloat16, and for a scheduler that
+# waits for every step's tokens, as it does where a repetition penalty is set: then the host's plan of a sharing step, 0.3 ms
+# longer, is on the step's path, and so much the layers have to save.  ms a step, ordinary against shared, at requests x shared
+# positions (MB a layer), waited for and in brackets run ahead: 8 x 4,096 (112) 4.00 and 4.15 (3.62 and 3.51), 16 x 2,048 (120) 4.11 and 4.35
+# (3.65 and 3.61), 32 x 1,328 (160) 4.59 and 4.90 (4.03 and 4.07), 20 x 2,160 (160) 4.74 and 4.96 (4.27 and 4.21), 16 x 2,752 (161) 4.24 and 4.33
+# (3.80 and 3.63); 6 x 8,192 (160) 4.35 and 4.33 (4.01 and 3.69), 8 x 5,888 (161) 4.19 and 4.20 (3.81 and 3.54), 12 x 4,096 (176) 4.43 and 4.44
+# (4.02 and 3.76), 8 x 8,192 (224) 4.44 and 4.24 (4.05 and 3.56), 16 x 4,096 (240) 4.57 and 4.42 (4.08 and 3.63), 32 x 2,048 (248) 4.92 and 4.98
+# (4.30 and 4.06), 64 x 1,024 (252) 5.80 and 5.99 (4.89 and 4.67), 8 x 16,384 5.62 and 4.50 (5.15 and 3.77), 64 x 8,192 12.1 and 6.5 (11.2 and 5.2).
+# Groups of fewer members gain little: 2 x 16,384 (67) 3.71 and 4.38 run ahead, 4 x 16,384 (201) 4.02 and 3.98.  Groups of other sizes and
+# models of other depths were not measured.
+WORTH_SHARING = 160 << 20
+FEW_SHARING = 12
 MEMBERS_WORTH_SHARING = 5
 # ... and in float32, where the other kernel gives every row a warp of its own: 8 heads in groups of 4, 2 x 64 (0.02 MB) 22 and 8 us,
 # 8 x 128 39 and 11, 8 x 2,048 566 and 13.

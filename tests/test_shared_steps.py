@@ -55,3 +55,12 @@ def test_the_same_batch_with_fewer_members(dtype):
                     assert first + (row0 + rows - 1) // 4 < 32 + live
         assert sorted(plan["members"][32 : 32 + live]) == list(range(live))
     assert len(sizes) == 1 and len(offsets) == 1
+
+
+@pytest.mark.parametrize("members,prefix,shares", [
+    (8, 4096, False), (16, 2048, False), (32, 1328, False), (20, 2160, False), (16, 2752, False), (64, 512, False), (4, 100_000, False),
+    (8, 6144, True), (12, 4096, True), (16, 4096, True), (32, 2048, True), (64, 8192, True), (5, 16384, True)])
+def test_a_step_shares_where_that_pays_for_its_plan(members, prefix, shares):
+    """8 key heads of 128 in groups of 4: shared where a step that the host waits for was no slower than the ordinary one."""
+    bucket = decode_bucket(members, 64, 64)
+    assert (SharedItems(4, 8, 128).step_plan(step_shape(bucket, members, prefix, 20)) is not None) == shares
