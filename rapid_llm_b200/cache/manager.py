@@ -322,7 +322,8 @@ class CacheManager:
         """Admit ``children`` as continuations of ``parent`` from where it is: the same tokens are cached, the pages they fill are
         shared (no one writes into those again), and each child gets a page of its own for the ragged last one.  Returns, per
         group, the ``(page of the parent, page of a child)`` copies that the device has to make before anyone writes on; ``None``
-        (and nothing taken) when slots or pages are short."""
+        (and nothing taken) when slots or pages are short.  A parent that shares with others still joins its children to that family,
+        whose number of shared positions stays: what the parent has cached since is held together but is no shared prefix."""
         held = self._get(parent)
         children = list(children)
         if len(set(children)) != len(children) or any(child in self._held for child in children):

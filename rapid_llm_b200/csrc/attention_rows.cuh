@@ -14,8 +14,8 @@
 //
 // By themselves, with the join: 64 requests of 8 key heads and 512 keys 27.8 us for 20.5 of HBM's rate, 2,048 keys 90 for 82,
 // 16 keys 6.6; heads of 64 (4 key heads) 2,048 keys 47 for 20.5: half the bytes in flight, so the loads' latency bounds them.
-// An item by itself takes 1.3 us a step of its warps.  Four CTAs a multiprocessor (126 registers) instead of three 43 ->
-// 40.5 us for 64 requests behind 8,192 shared keys; eight warps a CTA were slower, so were tiles by TMA into shared memory
+// An item by itself takes 1.3 us a step of its warps.  Four CTAs a multiprocessor (126 registers) instead of three took 6 %
+// off 64 requests behind 8,192 shared keys; eight warps a CTA were slower, so were tiles by TMA into shared memory
 // (13.5 -> 23 us for 16 requests behind 2,048) and the next step's keys ahead, for which the queries had to leave the
 // registers (27.8 -> 35.9 us for the 512 keys, heads of 64 16.2 -> 16.8).
 //

@@ -18,9 +18,11 @@
 // Measured: 2 us until the first copies are asked for, 2.7 for the queries, then 1.83 us a block for two tiles (0.95 of
 // softmax and 0.88 of products a tile, the tiles in strict turn: the tensor core, which reads Q or V from shared memory at its
 // full rate, is the longer half) or 0.98 us for one (104 CTAs and more then take all of HBM's rate), and 3.7 us to the results.
-// 64 requests, 32 heads on 8, 32,000 shared and 512 own keys: 58 us beside 21 of row items and 8 of the join; 8,192 keys: 28, 21 and
-// 6, one over the other 40.6, where each request for itself takes 220.  Tried and slower: scores of 64 keys a unit ahead (72 -> 87 us: Q is read as often for
-// 64 keys as for 128), a share of the exponentials as polynomials on the multiply-add pipes (-1 % to +8 %).
+// 64 requests, 32 heads on 8, 32,000 shared and 512 own keys: 58 us beside 21 of row items and 8 of the join; 8,192 keys and up to
+// 512 ragged own ones: 28, 21 and 7, one over the other 43, where each request for itself takes 220; 40 heads on 8, 32,000 and up to 1,024: 69 (320
+// rows: an item of 256 and one of 64 over each range, and the one of 64 takes as long a block), 31 and 7, one over the other 106.
+// Tried and slower: scores of 64 keys a unit ahead (72 -> 87 us: Q is read as often for 64 keys as for 128), a share of the
+// exponentials as polynomials on the multiply-add pipes (-1 % to +8 %).
 #pragma once
 
 #include "attention_prefill_tc.cuh"

@@ -525,7 +525,8 @@ sample_filtered_kernel(const Args args, unsigned ranks) {
   }
   __syncthreads();
   if (penalised) {
-    // every generated token once: the first of equal ids in the list applies the penalty
+    // every generated token once: the first of equal ids in the list applies the penalty.  (A walk of the list for each of the
+    // slice's tokens, so this grows with the square of what was generated.)
     for (int i = seen_begin + threadIdx.x; i < seen_end; i += kThreads) {
       const int id = args.seen_tokens[i] - row.begin;
       if (id < 0 || id >= row.count) continue;

@@ -202,7 +202,8 @@ class LLM:
 
         ``prompts``: a string, a list of strings, one list of token ids, or a list of them.
         ``sampling_params``: one set for all prompts, or one per prompt; ``n`` of them gives that many completions in
-        ``RequestOutput.outputs``, drawn from one computation of the prompt.
+        ``RequestOutput.outputs``, drawn from one computation of the prompt as far as slots and pages are free then; those
+        that find none compute it again.
         """
         encoded, requests = self._submit(prompts, sampling_params)
         self.scheduler.run_to_completion()

@@ -198,7 +198,8 @@ class ModelRunner:
 
     def compact(self) -> int:
         """Move every group's held pages to the lowest ids (steps that are enqueued keep theirs: the copies run behind
-        them); returns how many pages moved."""
+        them); returns how many pages moved.  For programs that look at the pages themselves (one contiguous range to save, say);
+        the engine never needs it, since any free page serves it."""
         moved = 0
         for group in range(len(self.cache.groups)):
             pairs = self.cache.compact(group)

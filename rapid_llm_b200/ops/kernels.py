@@ -1281,7 +1281,8 @@ def sample(
     ``counters``) given, a row keeps its ``top_k`` largest logits (of equal ones those of lowest index), of those what has
     at most ``top_p`` of their mass strictly above it, and of those what has at least ``min_p`` of the largest
     probability; the draw is the first index whose running kept mass exceeds ``u`` of all kept mass.  Masses are exact to 2^-43 of the
-    largest weight.  A row with ``temperature`` 0 takes the first maximum; one with ``top_k`` below 0 is passed over, its place in
+    largest weight; a draw of exactly 0 takes the first index that the cuts leave and whose weight is more than zero in float64,
+    however little that is.  A row with ``temperature`` 0 takes the first maximum; one with ``top_k`` below 0 is passed over, its place in
     ``out`` stays as it is.  Every array has one entry a row."""
     _need_cuda(logits, out, temperature, top_p, penalty, seeds, counters, seen_tokens, seen_offsets, top_k, min_p, uniforms)
     _expect("out", out, torch.int32)

@@ -339,6 +339,7 @@ class SharedItems(StepPlanner):
         elif not kernels.attention_tc_takes(self.head_dim, shape.page_size):
             tile_rows = kernels.CHUNK_TILE_ROWS
         else:
+            # one height for the whole step: beside items of more than 128 rows one of fewer takes as long a block as they do
             tile_rows = kernels.SHARED_TC_ROWS[int(work[:, 4].max()) > kernels.SHARED_TC_ROWS[0]]
         height = np.where(low, kernels.DECODE_TILE_ROWS, tile_rows)
         block = kernels.MMA_KEYS if self.wide else kernels.DECODE_TC_KEYS

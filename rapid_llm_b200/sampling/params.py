@@ -10,7 +10,8 @@ when the model folder has a tokenizer, and requests of token ids alone are never
 ``logprobs`` and ``prompt_logprobs`` (reporting, not sampling) are accepted only as ``None``;
 any other value is refused at construction rather than ignored.  Three more additions: ``top_k`` keeps the k largest
 logits before ``top_p`` is taken of what they leave (0 = all), ``min_p`` keeps what has at least that share of the largest
-probability (0 = everything), and ``n`` asks for several completions of one prompt, which is computed once for all of them.
+probability (0 = everything), and ``n`` asks for several completions of one prompt, which is computed once for all that find a slot and pages
+when it has been (the others compute it again, like requests of their own; so do all where it has one token).
 """
 
 from __future__ import annotations
